@@ -917,3 +917,8 @@ def router_gemm(x, w):
     out = torch.empty(T, E, dtype=torch.float32, device=x.device)
     _lib.check(_lib.lib().sb_router_gemm(P(x), P(w), P(out), T, K, E, _lib.stream()), "sb_router_gemm")
     return out
+
+
+# ---------------------------------------------------- drafted-token trees, logits before sampling
+from slime_b200.ops.tree import accept_tree, tree_attention  # noqa: E402, F401
+from slime_b200.ops.logits import adjust_logits  # noqa: E402, F401

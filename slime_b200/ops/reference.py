@@ -153,6 +153,112 @@ def paged_decode_attention(q, k_cache, v_cache, block_table, seq_lens, page_size
     return out
 
 
+def tree_ways(parents, cu_nodes) -> list[list[int]]:
+    """For every packed row of drafted-token trees the nodes from its own up to the root (numbers within the tree); empty for rows
+    that belong to no tree."""
+    par, cu = parents.tolist(), cu_nodes.tolist()
+    ways: list[list[int]] = [[] for _ in par]
+    for a, b in zip(cu[:-1], cu[1:]):
+        for i in range(b - a):
+            up = par[a + i]
+            if i == 0:
+                ways[a] = [0]
+            elif 0 <= up < i and ways[a + up]:
+                ways[a + i] = [i] + ways[a + up]
+    return ways
+
+
+def tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, parents, page_size, scale, sinks, out):
+    """Nodes of drafted-token trees over the cached context, the nodes above them and themselves (``ops.tree``)."""
+    Hq, Hkv = q.shape[1], k_cache.shape[1]
+    ways, cu = tree_ways(parents, cu_nodes), cu_nodes.tolist()
+    for b, (lo, hi) in enumerate(zip(cu[:-1], cu[1:])):
+        if hi == lo:
+            continue
+        ctx = int(context_lens[b])
+        pos = torch.arange(ctx + hi - lo, device=q.device)
+        slots = block_table[b, pos // page_size].long() * page_size + pos % page_size
+        sees = torch.zeros(hi - lo, ctx + hi - lo, dtype=torch.bool, device=q.device)
+        for i in range(hi - lo):
+            if ways[lo + i]:
+                sees[i, :ctx] = True
+                sees[i, [ctx + j for j in ways[lo + i]]] = True
+        ks = k_cache[slots].float().repeat_interleave(Hq // Hkv, dim=1)
+        vs = v_cache[slots].float().repeat_interleave(Hq // Hkv, dim=1)
+        vs = torch.where(sees.any(0)[:, None, None], vs, 0.0)
+        x = torch.einsum("ihd,jhd->hij", q[lo:hi].float() * scale, ks).masked_fill(~sees, float("-inf"))
+        if sinks is not None:
+            x = torch.cat([x, sinks.float()[:, None, None].expand(Hq, hi - lo, 1)], dim=-1)
+        p = torch.where(sees.any(1)[:, None], x.softmax(-1)[..., : sees.shape[1]], 0.0)
+        out[lo:hi] = torch.einsum("hij,jhd->ihd", p, vs).to(q.dtype)
+    return out
+
+
+def adjust_logits(logits, tokens, lengths, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, tree, out):
+    """Penalties, biases and masks on logits (``ops.adjust_logits``)."""
+    R, V = logits.shape
+    if tree is not None:
+        drafted, parents, cu_nodes = tree
+        ways, cu = tree_ways(parents, cu_nodes), cu_nodes.tolist()
+        owner = [b for b in range(len(cu) - 1) for _ in range(cu[b + 1] - cu[b])]
+    rows = []
+    for r in range(R):
+        if tree is not None and not cu[0] <= r < cu[-1]:
+            rows.append(out[r])
+            continue
+        b = r if tree is None else owner[r - cu[0]]
+        x = logits[r].float()
+        if repetition is not None or frequency is not None or presence is not None:
+            text = tokens[b, : int(lengths[b])].long()
+            answer = text[int(prompt_lens[b]) if prompt_lens is not None else 0 :]
+            if tree is not None:
+                more = torch.tensor([int(drafted[cu[b] + j]) for j in ways[r] if j > 0], dtype=torch.long, device=x.device)
+                text, answer = torch.cat([text, more]), torch.cat([answer, more])
+            inside = lambda t: t[(t >= 0) & (t < V)]  # noqa: E731
+            seen = torch.bincount(inside(text), minlength=V) > 0
+            used = torch.bincount(inside(answer), minlength=V).float()
+            if repetition is not None:
+                x = torch.where(seen, torch.where(x > 0, x / repetition[b], x * repetition[b]), x)
+            if frequency is not None:
+                x = torch.where(used > 0, x - frequency[b] * used, x)
+            if presence is not None:
+                x = torch.where(used > 0, x - presence[b], x)
+        if bias_ids is not None:
+            ids = bias_ids[b].long()
+            ok = (ids >= 0) & (ids < V)
+            x = x + torch.zeros_like(x).index_add_(0, ids[ok], bias_values[b][ok])
+        if allowed is not None:
+            t = torch.arange(V, device=x.device)
+            x = torch.where((allowed[r][t // 32] >> (t % 32)) & 1 > 0, x, float("-inf"))
+        rows.append(x.to(logits.dtype))
+    return torch.stack(rows) if rows else logits
+
+
+def accept_tree(sampled, drafted, parents, cu_nodes, max_nodes, caches, block_table, context_lens, page_size):
+    """The walk from the root along the sampled tokens; keys and values of its nodes move behind each other (``ops.tree``)."""
+    ways, cu = tree_ways(parents, cu_nodes), cu_nodes.tolist()
+    path = torch.full((len(cu) - 1, max_nodes), -1, dtype=torch.int32, device=sampled.device)
+    tokens, count = path.clone(), torch.zeros(len(cu) - 1, dtype=torch.int32, device=sampled.device)
+    said, guess = sampled.tolist(), drafted.tolist()
+    for b, (lo, hi) in enumerate(zip(cu[:-1], cu[1:])):
+        walk = [0] if hi > lo else []
+        while walk:
+            below = [j for j in range(1, hi - lo) if len(ways[lo + j]) > 1 and ways[lo + j][1] == walk[-1] and guess[lo + j] == said[lo + walk[-1]]]
+            if not below:
+                break
+            walk.append(below[0])
+        path[b, : len(walk)] = torch.tensor(walk, dtype=torch.int32)
+        tokens[b, : len(walk)] = torch.tensor([said[lo + i] for i in walk], dtype=torch.int32)
+        count[b] = len(walk)
+        if caches and walk:
+            at = torch.tensor([walk, list(range(len(walk)))], device=sampled.device) + int(context_lens[b])
+            src, dst = block_table[b, at // page_size].long() * page_size + at % page_size
+            for c in caches:
+                view = c if c.dim() == 4 else c[None]
+                view[:, dst] = view[:, src]
+    return path, tokens, count
+
+
 def logprob_entropy(logits, targets, inv_temperature=1.0):
     z = logits.float() * inv_temperature
     lse = torch.logsumexp(z, -1)

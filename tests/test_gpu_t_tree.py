@@ -1,0 +1,411 @@
+"""Operators of drafted-token trees and of logits before sampling on the GPU, against 64-bit loops (``tree_oracle``)."""
+
+import math
+
+import pytest
+import torch
+import tree_oracle as oracle
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16 = 2.0**-24, 2.0**-8  # half a step
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built(kernels):
+    yield
+
+
+def cuda(*ts):
+    return [None if t is None else t.cuda() for t in ts]
+
+
+def attention_case(sizes, ctx, heads, page, seed=0, holes=0.0, shape="random", dtype=torch.bfloat16, packed=False, spare=0):
+    """Caches are NaN wherever no token stands; the page table points far away behind a request's pages; ``spare`` rows of q follow the
+    last tree. ``packed``: q is a column range of a wider matrix, the caches are two halves of one tensor."""
+    Hq, Hkv, D = heads
+    g = torch.Generator().manual_seed(seed)
+    cu, parents = oracle.make_trees(sizes, seed, holes, shape)
+    table, slots = oracle.make_pages([c + n for c, n in zip(ctx, sizes)], page, seed)
+    T = int(cu[-1]) + spare
+    kv = torch.full((slots, 2, Hkv, D), math.nan).to(dtype)
+    for b, (c, n) in enumerate(zip(ctx, sizes)):
+        at = torch.tensor([oracle.slot(table, b, p, page) for p in range(c + n)], dtype=torch.long)
+        kv[at] = torch.randn(c + n, 2, Hkv, D, generator=g).to(dtype)
+    wide = (2 * torch.randn(T, Hq + 2, D, generator=g)).to(dtype)
+    if packed:
+        wide, kv = wide.cuda(), kv.cuda()
+        q, k, v = wide[:, 1:-1], kv[:, 0], kv[:, 1]
+    else:
+        q, k, v = wide[:, 1:-1].contiguous().cuda(), kv[:, 0].contiguous().cuda(), kv[:, 1].contiguous().cuda()
+    parents = torch.cat([parents, torch.zeros(spare, dtype=torch.int32)])
+    return q, k, v, *cuda(table, torch.tensor(ctx, dtype=torch.int32), cu, parents)
+
+
+def bound(want, mass, dtype, D):
+    """Scores are sums of D products, off by D roundings of fp32 of some 14 on this scale (1e-4) and by that factor in the weights; bf16 kernels round the weights
+    to bf16, and every kernel its output."""
+    weights = 1e-4 + (BF16 if dtype == torch.bfloat16 else 0)
+    return weights * mass + (BF16 if dtype == torch.bfloat16 else F32) * want.abs() + 1e-6
+
+
+SIZES = [
+    ([1], [0]),
+    ([1], [1]),
+    ([8], [1023]),
+    ([3, 1, 0, 17], [127, 128, 5, 129]),
+    ([16, 16, 16], [112, 0, 500]),
+    ([64, 5], [1000, 64]),
+    ([31, 61, 2], [97, 3, 255]),
+    ([128, 100], [40, 300]),
+    ([2] * 40, list(range(40))),
+]
+HEADS = [(14, 2, 64), (4, 4, 64), (32, 8, 128), (16, 1, 128), (8, 1, 128), (2, 2, 128)]
+
+
+@pytest.mark.parametrize("sizes, ctx", SIZES)
+@pytest.mark.parametrize("heads", HEADS)
+def test_attention_bf16(sizes, ctx, heads):
+    from slime_b200 import ops
+
+    q, k, v, table, c, cu, parents = attention_case(sizes, ctx, heads, 16, seed=len(sizes), holes=0.1 if len(sizes) > 1 else 0.0)
+    got = ops.tree_attention(q, k, v, table, c, cu, parents, 16, max(sizes))
+    want, mass = oracle.attention(q, k, v, table, c, cu, parents, 16, heads[2] ** -0.5)
+    err = (got.double().cpu() - want).abs()
+    assert (err <= bound(want, mass, torch.bfloat16, heads[2])).all(), float((err / (mass + 1e-9)).max())
+
+
+@pytest.mark.parametrize("heads, page", [((4, 2, 8), 4), ((6, 2, 80), 16), ((2, 1, 256), 32), ((3, 3, 5), 1), ((14, 2, 64), 16), ((8, 2, 128), 24)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_of_every_width_and_page(heads, page, dtype):
+    from slime_b200 import ops
+
+    q, k, v, table, c, cu, parents = attention_case([3, 1, 0, 17], [127, 128, 5, 40], heads, page, holes=0.1, dtype=dtype)
+    got = ops.tree_attention(q, k, v, table, c, cu, parents, page, 17)
+    want, mass = oracle.attention(q, k, v, table, c, cu, parents, page, heads[2] ** -0.5)
+    assert ((got.double().cpu() - want).abs() <= bound(want, mass, dtype, heads[2])).all()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 48])
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 8, 128)])
+def test_attention_strides_sinks_factors_and_pages(page, heads):
+    from slime_b200 import ops
+
+    q, k, v, table, c, cu, parents = attention_case([9, 1, 33], [300, 17, 65], heads, page, packed=True, spare=3)
+    sinks = torch.randn(heads[0], device="cuda")
+    for scale, s in ((None, sinks), (0.3, None), (-0.05, sinks), (0.0, None)):
+        out = torch.full(q.shape, 7.0, dtype=q.dtype, device="cuda")
+        assert ops.tree_attention(q, k, v, table, c, cu, parents, page, 33, scale=scale, sinks=s, out=out) is out
+        f = heads[2] ** -0.5 if scale is None else scale
+        want, mass = oracle.attention(q, k, v, table, c, cu, parents, page, f, s)
+        # (a factor of 0.3 makes scores of up to a hundred: their sums are off by as much more)
+        slack = 1 + abs(f) / heads[2] ** -0.5
+        n = int(cu[-1])
+        assert ((out[:n].double().cpu() - want[:n]).abs() <= slack * bound(want, mass, torch.bfloat16, heads[2])[:n]).all()
+        assert (out[n:] == 7).all()
+
+
+@pytest.mark.parametrize("shape", ["chain", "star"])
+def test_attention_of_chains_and_stars(shape):
+    from slime_b200 import ops
+
+    q, k, v, table, c, cu, parents = attention_case([70, 20], [60, 2000], (32, 8, 128), 16, shape=shape)
+    got = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 70)
+    want, mass = oracle.attention(q, k, v, table, c, cu, parents, 16, 128**-0.5)
+    assert ((got.double().cpu() - want).abs() <= bound(want, mass, torch.bfloat16, 128)).all()
+
+
+def test_attention_of_a_long_cache_and_empty_calls():
+    from slime_b200 import ops
+
+    q, k, v, table, c, cu, parents = attention_case([6, 12], [20011, 9000], (8, 2, 128), 16)
+    got = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 12)
+    want, mass = oracle.attention(q, k, v, table, c, cu, parents, 16, 128**-0.5)
+    assert ((got.double().cpu() - want).abs() <= bound(want, mass, torch.bfloat16, 128)).all()
+    assert ops.tree_attention(q[:0], k, v, table, c, torch.zeros_like(cu), parents[:0], 16, 12).shape == (0, 8, 128)
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert ops.tree_attention(q[:0], k, v, table[:0], c[:0], none, parents[:0], 16, 12).shape == (0, 8, 128)
+
+
+def test_attention_is_the_same_every_time_and_with_other_requests_beside_it_where_asked():
+    from slime_b200 import ops
+
+    q, k, v, table, c, cu, parents = attention_case([9] * 12, [400 + 37 * i for i in range(12)], (14, 2, 64), 16)
+    a = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 9)
+    for _ in range(3):
+        assert torch.equal(a, ops.tree_attention(q, k, v, table, c, cu, parents, 16, 9))
+    ops.set_batch_invariant(True)
+    try:
+        a = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 9)
+        for b in (0, 7):
+            lone = ops.tree_attention(q[9 * b : 9 * b + 9], k, v, table[b : b + 1], c[b : b + 1], cu[:2], parents[9 * b : 9 * b + 9], 16, 9)
+            assert torch.equal(lone, a[9 * b : 9 * b + 9])
+    finally:
+        ops.set_batch_invariant(False)
+
+
+def test_attention_on_another_stream_and_in_a_graph():
+    from slime_b200 import ops
+
+    q, k, v, table, c, cu, parents = attention_case([9, 30], [400, 77], (32, 8, 128), 16)
+    want = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 30)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 30)
+    side.synchronize()
+    assert torch.equal(want, other)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 30)
+    # other lengths and trees of the same packed rows
+    c.copy_(torch.tensor([390, 80], dtype=torch.int32))
+    cu[1] = 20
+    parents[9:20] = torch.arange(8, 19, dtype=torch.int32, device="cuda")
+    parents[20] = -1
+    q2 = q.clone()
+    q.mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    table_full = table.clone()
+    del q2
+    fresh = ops.tree_attention(q, k.nan_to_num(0.0), v.nan_to_num(0.0), table_full.clamp(max=k.shape[0] // 16 - 1), c, cu, parents, 16, 30)
+    assert fresh.isfinite().all()
+    assert torch.equal(held.nan_to_num(5.0)[:20], ops.tree_attention(q, k, v, table, c, cu, parents, 16, 30).nan_to_num(5.0)[:20])
+
+
+# -------------------------------------------------------------------------------------------------------------- logits
+def logits_case(S, V, sizes=None, seed=0, L=23, K=5, dtype=torch.float32, parts=("repetition", "frequency", "presence", "bias", "allowed")):
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.rand(*s, generator=g)  # noqa: E731
+    ints = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, dtype=torch.int32)  # noqa: E731
+    R = S if sizes is None else sum(sizes)
+    kw = dict(tokens=ints(-2, V + 2, S, L) // 3, lengths=ints(0, L + 1, S), prompt_lens=ints(0, L + 1, S))
+    if "repetition" in parts:
+        kw["repetition"] = 0.5 + rnd(S)
+    if "frequency" in parts:
+        kw["frequency"] = rnd(S) - 0.3
+    if "presence" in parts:
+        kw["presence"] = rnd(S) - 0.3
+    if "bias" in parts:
+        kw["bias_ids"], kw["bias_values"] = ints(-3, V + 3, S, K) // 2, torch.randn(S, K, generator=g)
+    if "allowed" in parts:
+        kw["allowed"] = torch.randint(-(1 << 31), 1 << 31, (R, -(-V // 32)), generator=g).to(torch.int32)
+        kw["allowed"][R // 2] = 0
+    if sizes is not None:
+        cu, parents = oracle.make_trees(sizes, seed, holes=0.1)
+        kw["tree"] = (ints(0, V, R), parents, cu)
+    x = 3 * torch.randn(R, V, generator=g)
+    x[0, 0], x[-1, V // 2], x[R // 2, -1] = 0.0, -math.inf, math.nan
+    dev = {n: tuple(t.cuda() for t in v) if isinstance(v, tuple) else v.cuda() for n, v in kw.items()}
+    return x.to(dtype), kw, dev
+
+
+def same_logits(got, want, dtype, spread=40):
+    # five roundings of fp32 of values below ``spread``, and of the result
+    half = BF16 if dtype == torch.bfloat16 else F32
+    torch.testing.assert_close(got.double().cpu(), want, rtol=half + 8 * F32, atol=8 * F32 * spread, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S, V, sizes, L, K", [(1, 1, None, 1, 1), (3, 31, None, 5, 40), (4, 4096, None, 300, 64), (3, 4097, [3, 0, 9], 1000, 7),
+                                               (2, 9001, [1, 128], 77, 1), (5, 12345, None, 4099, 700)])  # fmt: skip
+def test_logits(dtype, S, V, sizes, L, K):
+    from slime_b200 import ops
+
+    x, kw, dev = logits_case(S, V, sizes, L=L, K=K, dtype=dtype)
+    want, _ = oracle.adjusted(x, **kw)
+    y = x.cuda()
+    same_logits(ops.adjust_logits(y, **dev), want, dtype, spread=40 + K)
+    assert torch.equal(y.nan_to_num(9.0).cpu(), x.nan_to_num(9.0))
+    assert ops.adjust_logits(y, **dev, out=y) is y  # in place
+    same_logits(y, want, dtype, spread=40 + K)
+
+
+@pytest.mark.parametrize("parts", [(), ("repetition",), ("frequency",), ("presence",), ("bias",), ("allowed",)])
+def test_logits_parts_alone(parts):
+    from slime_b200 import ops
+
+    x, kw, dev = logits_case(6, 5003, parts=parts)
+    want, _ = oracle.adjusted(x, **kw)
+    same_logits(ops.adjust_logits(x.cuda(), **dev), want, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_strided_rows_and_rows_behind_the_last_tree(dtype):
+    from slime_b200 import ops
+
+    x, kw, dev = logits_case(3, 5003, [2, 3, 1], dtype=dtype)
+    drafted, parents, cu = dev["tree"]
+    pad = lambda t: torch.cat([t, t[:2]])  # noqa: E731
+    dev["tree"], dev["allowed"] = (pad(drafted), pad(parents), cu), pad(dev["allowed"])
+    want, _ = oracle.adjusted(x, **kw)
+    for left, right in ((1, 4), (0, 5), (3, 8)):  # rows that start and end off every boundary
+        wide = torch.full((8, left + 5003 + right), 7.0, dtype=dtype, device="cuda")
+        wide[:, left : left + 5003] = pad(x.cuda())
+        out = torch.full((8, 5003 + 2 * left), 5.0, dtype=dtype, device="cuda")[:, left : left + 5003]
+        ops.adjust_logits(wide[:, left : left + 5003], **dev, out=out)
+        same_logits(out[:6], want, dtype)
+        assert (out[6:] == 5).all()
+        ops.adjust_logits(wide[:, left : left + 5003], **dev, out=wide[:, left : left + 5003])
+        same_logits(wide[:6, left : left + 5003], want, dtype)
+        assert (wide[:, :left] == 7).all() and (wide[:, left + 5003 :] == 7).all()
+
+
+def test_logits_of_a_whole_vocabulary_in_a_graph():
+    from slime_b200 import ops
+
+    V, S = 151936, 3
+    x, kw, dev = logits_case(S, V, L=2000, parts=("repetition", "frequency", "presence", "bias"))
+    y = x.cuda()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.adjust_logits(y, **dev)
+    dev["tokens"].add_(11)
+    kw["tokens"] += 11
+    graph.replay()
+    want, _ = oracle.adjusted(x, **kw)
+    same_logits(out, want, torch.float32)
+    assert ops.adjust_logits(y[:0], allowed=torch.zeros(0, -(-V // 32), dtype=torch.int32, device="cuda")).shape == (0, V)
+
+
+# ------------------------------------------------------------------------------------------------------------- accept
+def accept_case(sizes, seed=0, share=0.8, holes=0.0):
+    g = torch.Generator().manual_seed(seed)
+    cu, parents = oracle.make_trees(sizes, seed, holes)
+    T = int(cu[-1])
+    drafted = torch.randint(0, 50, (T,), generator=g, dtype=torch.int32)
+    sampled = torch.randint(100, 200, (T,), generator=g, dtype=torch.int32)
+    for b in range(len(sizes)):
+        for i in range(1, sizes[b]):
+            up = int(parents[cu[b] + i])
+            if 0 <= up < i and torch.rand((), generator=g) < share:
+                sampled[cu[b] + up] = drafted[cu[b] + i]
+    return sampled, drafted, parents, cu
+
+
+@pytest.mark.parametrize("sizes", [[1], [8], [0, 5, 1, 0], [31, 32, 33], [128, 2], [3, 7] * 100])
+@pytest.mark.parametrize("shape", [(2, 1, 4), (3, 8, 128), (1, 3, 5), (2, 1, 3)])
+def test_acceptance(sizes, shape):
+    from slime_b200 import ops
+
+    layers, H, D = shape
+    for seed, share, holes in ((0, 1.0, 0.0), (1, 0.7, 0.2)):
+        ctx = [(7 * b + seed) % 40 for b in range(len(sizes))]
+        sampled, drafted, parents, cu = accept_case(sizes, seed, share, holes)
+        table, slots = oracle.make_pages([c + n for c, n in zip(ctx, sizes)], 16, seed)
+        caches = [torch.randn(layers, slots, H, D).bfloat16(), torch.randn(layers, slots, H, 2 * D).bfloat16()]
+        want = oracle.accepted(sampled, drafted, parents, cu, max(sizes))
+        after = oracle.moved(caches, table, ctx, [w[0] for w in want], [w[2] for w in want], 16)
+        dev = cuda(sampled, drafted, parents, cu)
+        at = dict(block_table=table.cuda(), context_lens=torch.tensor(ctx, dtype=torch.int32, device="cuda"), page_size=16)
+        for split in (False, True):
+            k, v = cuda(*caches)
+            path, tokens, count = ops.accept_tree(*dev, max(sizes), k_caches=list(k) if split else k, v_caches=list(v) if split else v, **at)
+            assert path.tolist() == [w[0] for w in want] and tokens.tolist() == [w[1] for w in want] and count.tolist() == [w[2] for w in want]
+            assert torch.equal(k.cpu(), after[0]) and torch.equal(v.cpu(), after[1])
+        alone = ops.accept_tree(*dev, max(sizes))
+        assert all(torch.equal(a, b) for a, b in zip(alone, (path, tokens, count)))
+
+
+def test_acceptance_of_many_layers_in_a_list_and_empty_values():
+    from slime_b200 import ops
+
+    sampled, drafted, parents, cu = accept_case([9, 12], 3, 1.0)
+    ctx = [15, 2]
+    table, slots = oracle.make_pages([c + n for c, n in zip(ctx, [9, 12])], 16, 0)
+    caches = [torch.randn(150, slots, 2, 8)]
+    want = oracle.accepted(sampled, drafted, parents, cu, 12)
+    after = oracle.moved(caches, table, ctx, [w[0] for w in want], [w[2] for w in want], 16)
+    k = caches[0].cuda()
+    ops.accept_tree(*cuda(sampled, drafted, parents, cu), 12, k_caches=list(k), v_caches=[torch.empty(slots, 1, 0, device="cuda")] * 150,
+                    block_table=table.cuda(), context_lens=torch.tensor(ctx, dtype=torch.int32, device="cuda"), page_size=16)  # fmt: skip
+    assert torch.equal(k.cpu(), after[0])
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    path, tokens, count = ops.accept_tree(none, none, none, torch.zeros(1, dtype=torch.int32, device="cuda"), 4)
+    assert path.shape == (0, 4) and count.shape == (0,)
+
+
+# ------------------------------------------------------------------------------------------------------- a whole round
+def test_a_round_of_drafted_trees_is_ordinary_decoding():
+    """One attention layer with a vocabulary behind it, in fp32 (close calls of the sampler aside, both forms then draw the same tokens): two rounds of trees, penalties included,
+    give the tokens that single steps give, and leave the cache that they leave."""
+    from slime_b200 import ops
+
+    g = torch.Generator().manual_seed(5)
+    V, Hq, Hkv, D, page, B = 97, 4, 2, 16, 16, 3
+    wq, wk, wv = (torch.randn(V, h * D, generator=g).cuda() for h in (Hq, Hkv, Hkv))
+    head = torch.randn(Hq * D, V, generator=g).cuda() * 0.4
+    ctx0 = [21, 3, 40]
+    texts = [torch.randint(0, V, (c + 1,), generator=g).tolist() for c in ctx0]
+    pens = dict(repetition=torch.tensor([1.3, 1.0, 0.8]).cuda(), frequency=torch.tensor([0.2, 0.0, 0.1]).cuda(), presence=torch.tensor([0.1, 0.0, 0.3]).cuda())
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, slots = oracle.make_pages([c + 64 for c in ctx0], page, 0)
+    dev_table = table.cuda()
+    prompts, seeds, temp = i32([c + 1 for c in ctx0]), torch.tensor([11, 12, 13], device="cuda"), torch.ones(B, device="cuda")
+
+    def fresh_cache():
+        k, v = torch.zeros(1, slots, Hkv, D, device="cuda"), torch.zeros(1, slots, Hkv, D, device="cuda")
+        for b in range(B):
+            at = torch.tensor([oracle.slot(table, b, p, page) for p in range(ctx0[b])], device="cuda")
+            ids = torch.tensor(texts[b][:-1], device="cuda")
+            k[0, at], v[0, at] = wk[ids].view(-1, Hkv, D), wv[ids].view(-1, Hkv, D)
+        return k, v
+
+    def step(k, v, text, ctx, sizes, parents, drafted):
+        """Feed the nodes, adjust and sample every row."""
+        cu = i32([0] + torch.tensor(sizes).cumsum(0).tolist())
+        ids, par, where = torch.tensor(drafted, device="cuda"), i32(parents), i32(ctx)
+        at = torch.tensor([oracle.slot(table, b, ctx[b] + i, page) for b in range(B) for i in range(sizes[b])], device="cuda")
+        k[0, at], v[0, at] = wk[ids].view(-1, Hkv, D), wv[ids].view(-1, Hkv, D)
+        o = ops.tree_attention(wq[ids].view(-1, Hq, D), k[0], v[0], dev_table, where, cu, par, page, max(sizes))
+        tokens = torch.zeros(B, 128, dtype=torch.int32)
+        for b in range(B):
+            tokens[b, : len(text[b])] = torch.tensor(text[b])
+        tree = (ids.int(), par, cu)
+        logits = ops.adjust_logits(o.view(-1, Hq * D) @ head, tokens.cuda(), i32([len(t) for t in text]), prompts, tree=tree, **pens)
+        # a node's place in the answer: behind the text, plus its depth
+        depth = [len(oracle.way_up(parents[int(cu[b]) : int(cu[b + 1])], i)) - 1 for b in range(B) for i in range(sizes[b])]
+        owner = [b for b in range(B) for _ in range(sizes[b])]
+        pos = i32([len(text[b]) - ctx0[b] - 1 + d for b, d in zip(owner, depth)])
+        rows = torch.tensor(owner, device="cuda")
+        tok = ops.sample(logits, temp[rows], seeds=seeds[rows], positions=pos)[0]
+        return tok, tree, where
+
+    # ordinary decoding: trees of one node
+    k1, v1 = fresh_cache()
+    plain = [list(t) for t in texts]
+    for n in range(14):
+        tok, _, _ = step(k1, v1, plain, [c + n for c in ctx0], [1] * B, [-1] * B, [t[-1] for t in plain])
+        for b, x in enumerate(tok.tolist()):
+            plain[b].append(x)
+    # two rounds: trees whose branches hold some right guesses and some wrong ones
+    k2, v2 = fresh_cache()
+    text, ctx = [list(t) for t in texts], list(ctx0)
+    moved = 0
+    for rnd in range(2):
+        sizes, parents, drafted = [6, 9, 4], [], []
+        for b in range(B):
+            good = plain[b][len(text[b]) :]
+            par = [-1, 0, 0, 2, 3, 1, 4, 2, 6][: sizes[b]] if rnd == 0 else [-1, 0, 1, 1, 3, 2, 4, 0, 6][: sizes[b]]
+            right = [0, 2, 3, 4, 6, 8] if rnd == 0 else [0, 1, 3, 4, 6, 8]
+            ids = [text[b][-1]] + [(good[0] + 17 + i) % V for i in range(1, sizes[b])]
+            for d, i in enumerate(right[1:]):
+                if i < sizes[b]:
+                    ids[i] = good[d]
+            parents += par
+            drafted += ids
+        tok, tree, where = step(k2, v2, text, ctx, sizes, parents, drafted)
+        path, new, count = ops.accept_tree(tok, tree[0], tree[1], tree[2], 9, k_caches=k2, v_caches=v2, block_table=dev_table, context_lens=where,
+                                           page_size=page)  # fmt: skip
+        for b in range(B):
+            n = int(count[b])
+            assert n >= 2
+            text[b] += new[b, :n].tolist()
+            ctx[b] += n
+            moved += sum(int(path[b, j]) != j for j in range(n))
+            assert text[b] == plain[b][: len(text[b])]
+    assert moved > 0
+    for b in range(B):
+        at = torch.tensor([oracle.slot(table, b, p, page) for p in range(ctx[b])], device="cuda")
+        assert torch.equal(k2[0, at], k1[0, at]) and torch.equal(v2[0, at], v1[0, at])
