@@ -63,7 +63,7 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
     if (tid == 0) found = -1;
     __syncthreads();
     for (int b = tid; b < a.requests; b += LG_THREADS)
-      if (a.cu[b] <= r && r < a.cu[b + 1]) found = b;
+      if (max(a.cu[b], 0) <= r && r < a.cu[b + 1]) found = b;
     __syncthreads();
     req = found;
     if (req < 0) return;  // behind the last tree: left as it is
@@ -89,7 +89,7 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
       }
     }
     if (a.cu != nullptr) {
-      const int first = a.cu[req], n = min(a.cu[req + 1] - first, TREE_MAX);
+      const int first = a.cu[req], n = min(min(a.cu[req + 1], a.rows) - first, TREE_MAX);
       for (int i = tid; i < n; i += LG_THREADS) {
         tree_p[i] = a.parents[first + i];
         tree_t[i] = a.drafted[first + i];

@@ -43,7 +43,7 @@ __device__ __forceinline__ void accept_move(const AcceptSlabs& c, const int* src
 
 __global__ void __launch_bounds__(AC_THREADS)
 tree_accept_kernel(const int* __restrict__ sampled, const int* __restrict__ drafted, const int* __restrict__ parents,
-                   const int* __restrict__ cu, int* __restrict__ path, int* __restrict__ tokens, int* __restrict__ count, int max_nodes,
+                   const int* __restrict__ cu, int* __restrict__ path, int* __restrict__ tokens, int* __restrict__ count, int rows, int max_nodes,
                    const __grid_constant__ AcceptSlabs slabs, const int* __restrict__ table, const int* __restrict__ context,
                    int page_size, int max_pages, int writes) {
   __shared__ int way[TREE_MAX], said[TREE_MAX];
@@ -52,7 +52,7 @@ tree_accept_kernel(const int* __restrict__ sampled, const int* __restrict__ draf
   pdl_wait();
   pdl_launch_dependents();
   const int b = blockIdx.x, lane = threadIdx.x & 31;
-  const int first = cu[b], n = min(max(cu[b + 1] - first, 0), max_nodes);
+  const int first = cu[b], n = first < 0 ? 0 : min(max(min(cu[b + 1], rows) - first, 0), max_nodes);
   if (threadIdx.x < 32) {
     int up[4], draft[4];
 #pragma unroll
@@ -129,7 +129,7 @@ tree_accept_kernel(const int* __restrict__ sampled, const int* __restrict__ draf
 
 // path, tokens: [B, max_nodes], -1 behind the accepted nodes; count: [B] (all three are written when `writes`). bases: n_bases addresses, each the
 // first of `layers` slabs that lie `step` bytes apart; rows of row_units * unit bytes, row_bytes apart. n_bases 0: nothing is moved.
-extern "C" int sb_tree_accept(const int* sampled, const int* drafted, const int* parents, const int* cu, int* path, int* tokens, int* count, int B,
+extern "C" int sb_tree_accept(const int* sampled, const int* drafted, const int* parents, const int* cu, int* path, int* tokens, int* count, int rows, int B,
                               int max_nodes, const void* bases, int n_bases, int layers, long step, int slots, int row_units, int unit,
                               long row_bytes, const int* table, const int* context, int page_size, int max_pages, int writes, int sms,
                               cudaStream_t s) {
@@ -150,5 +150,5 @@ extern "C" int sb_tree_accept(const int* sampled, const int* drafted, const int*
   const long want = (4L * sms + B - 1) / B;
   const int parts = static_cast<int>(all < 1 ? 1 : (all < want ? all : want));
   return (int)sb::launch_pdl(sb::tree_accept_kernel, dim3(B, parts), dim3(sb::AC_THREADS), 0, s, sampled, drafted, parents, cu, path, tokens, count,
-                             max_nodes, c, table, context, page_size, max_pages, writes);
+                             rows, max_nodes, c, table, context, page_size, max_pages, writes);
 }

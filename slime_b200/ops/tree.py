@@ -22,10 +22,12 @@ whatever was drafted. CPU tensors run the definitions in ``reference``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
 
+from slime_b200 import ops
 from slime_b200.ops import _checks, _lib, reference
 
 P = _lib.ptr
@@ -56,6 +58,14 @@ def check_trees(op: str, rows: int, cu_nodes, max_nodes: int, **per_node):
     if _checks.enabled():
         _checks.index_range(op, "cu_nodes", cu_nodes, upper=rows + 1)
         _checks.index_range(op, "tree sizes", cu_nodes[1:] - cu_nodes[:-1], upper=max_nodes + 1)
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(B: int, Hq: int, Hkv: int, D: int, max_nodes: int, tokens: int, whole: int, sms: int) -> int:
+    """Bytes of workspace of the tensor-core kernel; -1 where it does not cover the call."""
+    ctas, tiles, size = ctypes.c_int(), ctypes.c_int(), ctypes.c_long()
+    rc = _lib.lib().sb_tree_attn_plan(B, Hq, Hkv, D, max_nodes, tokens, whole, sms, ctypes.byref(ctas), ctypes.byref(tiles), ctypes.byref(size))
+    return size.value if rc == 0 else -1
 
 
 def tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, parents, page_size: int, max_nodes: int, scale=None,
@@ -103,7 +113,21 @@ def tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, par
         with torch.cuda.device(q.device):
             return tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, parents, page_size, max_nodes, scale, sinks, out)
     q, k_cache, v_cache = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k_cache, v_cache))
-    rc = _lib.lib().sb_tree_attn(
+    lib = _lib.lib()
+    if q.dtype == torch.bfloat16 and scale > 0:
+        whole, sms = int(ops.BATCH_INVARIANT), _lib.sm_count(q.device)
+        size = _workspace(B, Hq, Hkv, D, max_nodes, block_table.shape[1] * page_size, whole, sms)
+        if size >= 0:
+            work = torch.empty(size, dtype=torch.uint8, device=q.device)
+            rc = lib.sb_tree_attn_tc(
+                P(q), P(k_cache), P(v_cache), P(block_table), P(context_lens), P(cu_nodes), P(parents), P(sinks), P(out), T, B, Hq, Hkv, D,
+                page_size, block_table.shape[1], k_cache.shape[0], max_nodes, q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1),
+                v_cache.stride(0), v_cache.stride(1), out.stride(0), scale, whole, P(work), size, sms, P(_lib.status_word(q.device)),
+                _lib.stream())  # fmt: skip
+            if rc != -1:
+                _lib.check(rc, "sb_tree_attn_tc", 2 - whole)
+                return out
+    rc = lib.sb_tree_attn(
         P(q), P(k_cache), P(v_cache), P(block_table), P(context_lens), P(cu_nodes), P(parents), P(sinks), P(out), T, B, Hq, Hkv, D,
         page_size, block_table.shape[1], k_cache.shape[0], max_nodes, q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1),
         v_cache.stride(0), v_cache.stride(1), out.stride(0), scale, int(q.dtype == torch.float32), _lib.stream())  # fmt: skip
@@ -171,7 +195,7 @@ def accept_tree(sampled, drafted, parents, cu_nodes, max_nodes: int, *, k_caches
         for i in range(0, max(1, len(bases)), 128):
             part = bases[i : i + 128]
             rc = _lib.lib().sb_tree_accept(
-                P(sampled), P(drafted), P(parents), P(cu_nodes), P(path), P(tokens), P(count), B, max_nodes,
+                P(sampled), P(drafted), P(parents), P(cu_nodes), P(path), P(tokens), P(count), T, B, max_nodes,
                 (ctypes.c_ulonglong * len(part))(*part), len(part), layers, step, slots, width // unit, unit, pitch, P(block_table),
                 P(context_lens), page_size or 1, 0 if block_table is None else block_table.shape[1], int(first), sms, stream)  # fmt: skip
             _lib.check(rc, "sb_tree_accept")
