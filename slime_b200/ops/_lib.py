@@ -96,7 +96,7 @@ _SIGS = {
     "sb_sample": [P, I, L, I, I, P, P, P, P, P, P, P, P, P, P, I, P],
     "sb_tree_attn": [P] * 9 + [I] * 9 + [L] * 7 + [F, I, P],
     "sb_adjust_logits": [P] * 14 + [L] * 5 + [I] * 6 + [P],
-    "sb_tree_attn_plan": [I, I, I, I, I, L, I, I, P, P, P],
+    "sb_tree_attn_plan": [I, I, I, I, I, L, I, I, P],
     "sb_tree_attn_tc": [P] * 9 + [I] * 9 + [L] * 7 + [F, I, P, L, I, P, P],
     "sb_tree_accept": [P, P, P, P, P, P, P, I, I, I, P, I, I, L, I, I, I, L, P, P, I, I, I, I, P],
     "sb_kv_write": [P, P, P, P, P, I, I, I, I, P],

@@ -63,8 +63,8 @@ def check_trees(op: str, rows: int, cu_nodes, max_nodes: int, **per_node):
 @functools.lru_cache(maxsize=4096)
 def _workspace(B: int, Hq: int, Hkv: int, D: int, max_nodes: int, tokens: int, whole: int, sms: int) -> int:
     """Bytes of workspace of the tensor-core kernel; -1 where it does not cover the call."""
-    ctas, tiles, size = ctypes.c_int(), ctypes.c_int(), ctypes.c_long()
-    rc = _lib.lib().sb_tree_attn_plan(B, Hq, Hkv, D, max_nodes, tokens, whole, sms, ctypes.byref(ctas), ctypes.byref(tiles), ctypes.byref(size))
+    size = ctypes.c_long()
+    rc = _lib.lib().sb_tree_attn_plan(B, Hq, Hkv, D, max_nodes, tokens, whole, sms, ctypes.byref(size))
     return size.value if rc == 0 else -1
 
 
