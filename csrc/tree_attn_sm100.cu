@@ -296,81 +296,87 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     } else if (warp == 1) {
       // -------------------------------------------------------------------- MMA issuer
       // Per group one step at a time: scores, then (once P is there) the product, then the next step's scores, which may be the next piece's.
-      if (lane == 0) {
-        constexpr uint32_t idesc_s = make_idesc(128, TT_BN, 1, 1, 0, 0);
-        constexpr uint32_t idesc_o = make_idesc(128, D, 1, 1, 0, 1);  // A = P in TMEM, B = V read MN-major
-        const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, UMMA_SWIZZLE_128B);
-        const uint64_t k_desc = make_smem_desc(smem_u32(sKV), 16, 1024, UMMA_SWIZZLE_128B);
-        const uint64_t v_desc = make_smem_desc(smem_u32(sKV), TT_BN * 128, 1024, UMMA_SWIZZLE_128B);
-        bool ok = true, more = walk.next(a);
-        uint32_t half0 = 0, piece = 0, p_cnt[2] = {0, 0};
-        int j = 0, second = 0;  // the next scores: tile of the piece, and whether they are the second query tile's
-        struct Step {
-          uint32_t v_half, piece;
-          bool there, first, last, frees;
-        } step[2];
-        auto wait_half = [&](uint32_t h) {
-          ok = ok && mbar_wait(&full[h % S::RING], (h / S::RING) & 1, cta_abort, status, ERR_WAIT_FULL);
-          if (ok) tc_fence_after();
-        };
-        auto scores = [&](int g) {
-          step[g].there = false;
-          if (!more) return;
-          const int nt = walk.nt;
-          const bool rows2 = TILES == 2 && walk.groups == 2;
-          if (j == 0 && !second) ok = ok && mbar_wait(q_full, piece & 1, cta_abort, status, ERR_WAIT_FULL);
-          const uint32_t kh = half0 + (j == 0 ? 0 : 2 * j - 1);
-          if (!second) wait_half(kh);
-          if (!ok) return;
-          const uint64_t qd = q_desc + second * (S::Q_TILE >> 4), kd = k_desc + (kh % S::RING) * (S::KV_TILE >> 4);
+      // The whole warp goes through it with the same values; one lane issues.
+      constexpr uint32_t idesc_s = make_idesc(128, TT_BN, 1, 1, 0, 0);
+      constexpr uint32_t idesc_o = make_idesc(128, D, 1, 1, 0, 1);  // A = P in TMEM, B = V read MN-major
+      const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, UMMA_SWIZZLE_128B);
+      const uint64_t k_desc = make_smem_desc(smem_u32(sKV), 16, 1024, UMMA_SWIZZLE_128B);
+      const uint64_t v_desc = make_smem_desc(smem_u32(sKV), TT_BN * 128, 1024, UMMA_SWIZZLE_128B);
+      bool ok = true, more = walk.next(a);
+      uint32_t half0 = 0, piece = 0, p_cnt[2] = {0, 0};
+      int j = 0, second = 0;  // the next scores: tile of the piece, and whether they are the second query tile's
+      struct Step {
+        uint32_t v_half, piece;
+        bool there, first, last, frees;
+      } step[2];
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        ok = ok && mbar_wait(bar, parity, cta_abort, status, code);
+        ok = __all_sync(0xffffffffu, ok);
+      };
+      auto scores = [&](int g) {
+        step[g].there = false;
+        if (!more) return;
+        const int nt = walk.nt;
+        const bool rows2 = TILES == 2 && walk.groups == 2;
+        const uint32_t kh = half0 + (j == 0 ? 0 : 2 * j - 1);
+        if (!second) {
+          if (j == 0) wait(q_full, piece & 1, ERR_WAIT_FULL);
+          wait(&full[kh % S::RING], (kh / S::RING) & 1, ERR_WAIT_FULL);
+        }
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t qd = q_desc + second * (S::Q_TILE >> 4), kd = k_desc + (kh % S::RING) * (S::KV_TILE >> 4);
+        const bool done = !rows2 || second, last = done && j + 1 == nt;
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const int at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
             umma_f16(tmem_base + g * TT_BN, qd + at, kd + at, idesc_s, k != 0 ? 1u : 0u);
           }
           umma_commit(&s_full[g]);
-          step[g].there = true;
-          step[g].piece = piece;
-          step[g].v_half = half0 + (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1);
-          step[g].first = rows2 ? j == 0 : j < 2;
-          step[g].last = rows2 ? j + 1 == nt : j + 2 >= nt;
-          step[g].frees = !rows2 || second;
-          if (!rows2 || second) {
-            umma_commit(&empty[kh % S::RING]);
-            second = 0;
-            if (++j == nt) {
-              umma_commit(q_empty);
-              half0 += 2 * nt;
-              j = 0;
-              ++piece;
-              more = walk.next(a);
-            }
-          } else {
-            second = 1;
-          }
-        };
-        scores(0);
-        if (ok) scores(1);
-        auto run = [&](int g) -> bool {
-          if (!ok || !step[g].there) return false;
-          ok = mbar_wait(&p_full[g], p_cnt[g]++ & 1, cta_abort, status, ERR_WAIT_TMEM_EMPTY);
-          wait_half(step[g].v_half);
-          // (the accumulators of the last piece have been read)
-          if (step[g].first) ok = ok && mbar_wait(o_empty, (step[g].piece & 1) ^ 1, cta_abort, status, ERR_WAIT_TMEM_EMPTY);
-          if (!ok) return false;
-          tc_fence_after();
-          const uint64_t vd = v_desc + (step[g].v_half % S::RING) * (S::KV_TILE >> 4);
-          const bool first = step[g].first;
+          if (done) umma_commit(&empty[kh % S::RING]);
+          if (last) umma_commit(q_empty);
+        }
+        __syncwarp();
+        step[g].there = true;
+        step[g].piece = piece;
+        step[g].v_half = half0 + (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1);
+        step[g].first = rows2 ? j == 0 : j < 2;
+        step[g].last = rows2 ? j + 1 == nt : j + 2 >= nt;
+        step[g].frees = done;
+        second = !done;
+        if (last) {
+          half0 += 2 * nt;
+          j = 0;
+          ++piece;
+          more = walk.next(a);
+        } else if (done) {
+          ++j;
+        }
+      };
+      auto run = [&](int g) -> bool {
+        if (!ok || !step[g].there) return false;
+        wait(&p_full[g], p_cnt[g]++ & 1, ERR_WAIT_TMEM_EMPTY);
+        wait(&full[step[g].v_half % S::RING], (step[g].v_half / S::RING) & 1, ERR_WAIT_FULL);
+        if (step[g].first) wait(o_empty, (step[g].piece & 1) ^ 1, ERR_WAIT_TMEM_EMPTY);  // (the accumulators of the last piece have been read)
+        if (!ok) return false;
+        tc_fence_after();
+        const uint64_t vd = v_desc + (step[g].v_half % S::RING) * (S::KV_TILE >> 4);
+        const bool first = step[g].first;
+        if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < TT_BN / 16; ++k)
             umma_f16_ts(tmem_base + 2 * TT_BN + g * D, tmem_base + g * TT_BN + k * 8, vd + k * (2048 >> 4), idesc_o, (!first || k != 0) ? 1u : 0u);
           if (step[g].frees) umma_commit(&empty[step[g].v_half % S::RING]);
           if (step[g].last) umma_commit(&o_full[g]);
-          scores(g);
-          return ok;
-        };
-        while (run(0) && run(1)) {
         }
+        __syncwarp();
+        scores(g);
+        return ok;
+      };
+      scores(0);
+      scores(1);
+      while (run(0) && run(1)) {
       }
     } else if (warp == 10) {
       // -------------------------------------------------------------------- queries and ways up, a piece ahead of the others
@@ -473,7 +479,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             // A row of 128 columns is read twice, in quarters: for its maximum the last two, then the first two, which stay in
             // registers; the last two come back behind those (P takes the columns of the first two only).
             uint32_t ra[32], rb[32];
-            float mx;
+            float mx = -INFINITY;
             const int x0 = copy * (COLS / 32);
             if constexpr (COLS == 128) {
               tmem_ld_32x32(s_addr + 64, ra);
@@ -493,7 +499,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               if constexpr (COLS > 32) hide(rb, x0 + 1);
             }
             const float m01 = COLS > 32 ? fmaxf(top(ra), top(rb)) : top(ra);
-            mx = (COLS == 128 ? fmaxf(mx, m01) : m01) * a.c_log2;  // c > 0: the maximum commutes with the scaling
+            mx = fmaxf(mx, m01) * a.c_log2;  // c > 0: the maximum commutes with the scaling
             const float m_new = fmaxf(m_run, mx);
             if (i == 0) {
               m_run = m_new;
