@@ -8,18 +8,23 @@
 //   P_g  = 2^(S_g c - m)      TMEM -> registers -> bf16 over the scores it came from (the A operand of the next product)
 //   O_g += P_g V_j            M 128, N D, K 128       TMEM
 //
-// One CTA per SM: warp 0 issues TMA loads (a box per page and 64-wide chunk), warp 1 the products, and two groups of four softmax warps
-// have one row per thread. Where a tree fits one tile the groups take the even and the odd key tiles, as if the keys were split between
-// two launches, each with its own maximum, sum and accumulator, and the epilogue joins the two; larger trees give each group
+// One CTA per SM: warps 0 and 3 issue TMA loads (a box per page and 64-wide chunk), warps 1 and 2 the products of one group each, and two
+// groups of four softmax warps have one row per thread. Where a tree fits one tile the groups take key tiles in turn, as if the keys were
+// split between two launches, each with its own maximum, sum and accumulator, and the epilogue joins the two; larger trees give each group
 // a query tile. Either way one group's softmax runs beside the other's products.
+//
+// What bounds a tile is the time of a warp's softmax over its columns, not the tensor cores: so a tree of up to 64 (32) rows is put into its
+// tile 2 (4) times, and each copy takes half (a quarter) of the columns, with maximum and sum of its own and zeros as weights of the others'
+// columns. The copies' accumulators are joined like the groups' are.
 //
 // Equal shares: the key tiles of all (request, query tile pair, kv head) items are numbered through, and CTA c takes the c-th of gridDim
 // equal ranges, whatever the lengths are. A range that begins or ends inside an item leaves that part's O, m, l in a workspace, and a
 // second launch joins the parts in order: the same bits on every run. With `whole` each CTA takes one item, so that a row's arithmetic does
 // not depend on the batch.
 //
-// K and V tiles share one ring in the order K0, K1, V0, K2, V1, ..., the order in which they are used, and the ring runs on from one piece
-// of work to the next. The scores of hidden nodes become -infinity by a bit mask per row, looked at in the last tiles only. Cache rows behind
+// Key and value tiles have a ring of buffers each, with a producer of its own, and the rings run on from one piece of work to the next. Every
+// waiter sees every phase of a barrier: a wait by parity cannot tell one phase from the next but one. Even rings give that to the groups, which
+// take tiles in turn; a ring of three buffers has six barriers for it; with two query tiles one warp waits for both groups. The scores of hidden nodes become -infinity by a bit mask per row, looked at in the last tiles only. Cache rows behind
 // the last node may hold anything: pages behind it are fetched from outside the cache, which reads as zero, and the rest of its page is
 // cleared in shared memory before the product of weights (zero) and values.
 // Every wait is bounded: on expiry the CTA records a status word, drains and returns with its TMEM freed.
@@ -29,7 +34,7 @@
 
 namespace sb {
 
-constexpr int TT_THREADS = 352;
+constexpr int TT_THREADS = 384;
 constexpr int TT_BN = 128;
 
 template <int D, int TILES, int REP>
@@ -37,7 +42,8 @@ struct TtSmem {
   static constexpr int NCH = D / 64;                 // 128-byte chunks of the head dim
   static constexpr int Q_TILE = 128 * 128 * NCH;
   static constexpr int KV_TILE = TT_BN * 128 * NCH;  // one K or V tile
-  static constexpr int RING = D == 64 ? 10 : (TILES == 1 ? 5 : 4);
+  static constexpr int K_RING = D == 64 ? 4 : 2, V_RING = D == 64 ? 6 : (TILES == 1 ? 3 : 2), RING = K_RING + V_RING;
+  static constexpr int V_FULL = V_RING % 2 == 0 ? V_RING : 2 * V_RING;  // barriers of values that have come
   static constexpr int RED = REP > 1 ? 2 * 128 * 80 : 0;  // [2 groups][128 rows][16 columns + 4]: sums over the copies
   static constexpr int TABLE = (TT_THREADS * 12 + 15) / 16 * 16;
   // behind the ring: ways up [2 pieces][128 nodes], (m, l) [2 pieces][2 groups][128 rows], parents [128], requests, barriers
@@ -147,8 +153,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   TtRequest* near = reinterpret_cast<TtRequest*>(par + 128);
   uint64_t* q_full = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(near) + S::TABLE);
   uint64_t* q_empty = q_full + 1;
-  uint64_t* full = q_empty + 1;    // [RING]
-  uint64_t* empty = full + S::RING;
+  uint64_t* full = q_empty + 1;    // [K_RING + V_FULL]
+  uint64_t* empty = full + S::K_RING + S::V_FULL;  // [RING]
   uint64_t* s_full = empty + S::RING;  // [2] scores of the group are there, and every product issued before them is done
   uint64_t* p_full = s_full + 2;       // [2] the group's P is in TMEM (4 arrivals)
   uint64_t* o_full = p_full + 2;       // [2] the group's last product of the piece is done
@@ -158,17 +164,15 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(w_empty + 2);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 2);  // [0] request, [1] unit within it
-  int* sums = start + 2;                               // [11] units of the warps' requests
+  int* sums = start + 2;                               // [12] units of the warps' requests
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* status = a.status;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
-    for (int s = 0; s < S::RING; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
+    mbar_init(q_empty, 2);  // one arrival per issuing warp
+    for (int s = 0; s < S::K_RING + S::V_FULL; ++s) mbar_init(&full[s], 1);
+    for (int s = 0; s < S::RING; ++s) mbar_init(&empty[s], 2);
     for (int g = 0; g < 2; ++g) {
       mbar_init(&s_full[g], 1);
       mbar_init(&p_full[g], 4);
@@ -249,181 +253,211 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     walk.look(a);
     const int page = 1 << a.page_shift, pages = TT_BN >> a.page_shift;  // of a tile
 
-    // A piece's tiles go to the two groups in turn, and the turn runs on from piece to piece: with one query tile, key tile j belongs to group
-    // (turn + j) & 1; with two, the first one belongs to group turn & 1 and takes its turn before the other.
-    if (warp == 0) {
-      // -------------------------------------------------------------------- TMA producer (lane p: page p of the tile)
+    // Steps go to the two groups in turn, and the turn runs on from piece to piece: with one query tile, key tile j of a piece belongs to group
+    // (turn + j) & 1; with two, every key tile is a step of both, and group turn & 1 has the first query tile. t0: the CTA's key tiles before a piece.
+    if (warp == 0 || warp == 3) {
+      // -------------------------------------------------------------------- TMA producers: keys, and values with queries and ways up
+      // (lane p: page p of the tile). Issuing a box costs a warp some 100 cycles, so keys and values have a warp each.
+      const bool is_k = warp == 0;
+      const CUtensorMap* map = is_k ? &tmK : &tmV;
       bool ok = true;
-      uint32_t half = 0;  // halves issued so far
-      int pieces = 0;
-      auto fetch = [&](const CUtensorMap* map, int slot0) {
-        const uint32_t st = half % S::RING;
-        if (lane == 0) {
-          ok = mbar_wait(&empty[st], ((half / S::RING) & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
-          if (ok) mbar_arrive_expect_tx(&full[st], S::KV_TILE);
-        }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        if (ok && lane < pages)
-#pragma unroll
-          for (int ch = 0; ch < NCH; ++ch)
-            tma_load_3d(sKV + st * S::KV_TILE + ch * (TT_BN * 128) + lane * page * 128, map, &full[st], ch * 64, walk.kvh, slot0);
-        ++half;
-      };
-      while (ok && walk.next(a)) {
+      uint32_t t0 = 0;  // tiles of the pieces before
+      for (uint32_t piece = 0; ok && walk.next(a); ++piece) {
+        const int nt = walk.nt;
         const int* row = a.table + static_cast<long>(walk.b) * a.max_pages;
         // a page behind the last key is fetched from behind the cache: zeros
         auto slot_of = [&](int j) {
           const int key = (walk.tile0 + j) * TT_BN + lane * page;
-          return j < walk.nt && lane < pages && key < walk.keys ? row[key >> a.page_shift] << a.page_shift : a.num_slots;
+          return j < nt && lane < pages && key < walk.keys ? row[key >> a.page_shift] << a.page_shift : a.num_slots;
         };
-        int s0 = slot_of(0), s1 = slot_of(1);
-        if (lane == 0 && walk.tile0 == 0 && walk.nt < walk.tiles) {  // the item goes on in the CTAs behind this one
-          const int last = walk.u - walk.nt + walk.tiles - 1;         // unit of its last tile, and the CTA that has it
-          const int owner = last < rest * (per + 1) ? last / (per + 1) : rest + (last - rest * (per + 1)) / per;
-          a.plan[2 * c] = make_int4(owner - c + 1, 2 * c + (pieces == 0 ? 0 : 1), walk.kvh, walk.pair * TILES * a.bq);
-          a.plan[2 * c + 1] = make_int4(walk.r.first, walk.r.n, 0, 0);
+        int slot0 = slot_of(0), slot1 = slot_of(1);
+        if (is_k) {
+          if (lane == 0 && walk.tile0 == 0 && nt < walk.tiles) {      // the item goes on in the CTAs behind this one
+            const int last = walk.u - nt + walk.tiles - 1;            // unit of its last tile, and the CTA that has it
+            const int owner = last < rest * (per + 1) ? last / (per + 1) : rest + (last - rest * (per + 1)) / per;
+            a.plan[2 * c] = make_int4(owner - c + 1, 2 * c + (piece == 0 ? 0 : 1), walk.kvh, walk.pair * TILES * a.bq);
+            a.plan[2 * c + 1] = make_int4(walk.r.first, walk.r.n, 0, 0);
+          }
+        } else {
+          const uint32_t buf = piece & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&w_empty[buf], ((piece >> 1) & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY));
+          if (!ok) break;
+          const bool hides = (walk.tile0 + nt) * TT_BN > walk.r.ctx;  // the piece has keys of nodes
+          if (hides) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+              if (x * 32 + lane < walk.r.n) par[x * 32 + lane] = a.parents[walk.r.first + x * 32 + lane];
+          }
+          if (lane == 0) {
+            ok = mbar_wait(q_empty, (piece & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
+            if (ok) {
+              mbar_arrive_expect_tx(q_full, (REP > 1 ? REP : walk.groups) * a.bq * a.G * 128 * NCH);
+              const int row0 = walk.r.first + walk.pair * TILES * a.bq;
+              // two query tiles, or copies of one
+              for (int x = 0; x < (REP > 1 ? REP : walk.groups); ++x)
+#pragma unroll
+                for (int ch = 0; ch < NCH; ++ch)
+                  tma_load_3d(sQ + x * (REP > 1 ? ROWS * 128 : S::Q_TILE) + ch * (128 * 128), &tmQ, q_full, ch * 64, walk.kvh * a.G,
+                              row0 + (REP > 1 ? 0 : x * a.bq));
+            }
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (!ok) break;
+          if (hides) {
+            __syncwarp();
+            for (int i = lane; i < walk.r.n; i += 32) {
+              uint32_t set[4];
+              tree_way_up([&](int j) { return par[j]; }, i, set);
+              ways[buf * 128 + i] = make_uint4(set[0], set[1], set[2], set[3]);
+            }
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&w_full[buf]);
         }
-        ++pieces;
-        fetch(&tmK, s0);
-        for (int j = 0; j < walk.nt && ok; ++j) {
-          const int s2 = slot_of(j + 2);
-          if (j + 1 < walk.nt) fetch(&tmK, s1);
-          if (ok) fetch(&tmV, s0);
-          s0 = s1;
-          s1 = s2;
+        for (int j = 0; j < nt; ++j) {
+          const int slot2 = slot_of(j + 2);
+          const uint32_t ring = is_k ? S::K_RING : S::V_RING, t = t0 + j, st = t % ring + (is_k ? 0 : S::K_RING);
+          uint64_t* come = &full[is_k ? st : S::K_RING + t % S::V_FULL];
+          if (lane == 0) {
+            ok = mbar_wait(&empty[st], (t / ring & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
+            if (ok) mbar_arrive_expect_tx(come, S::KV_TILE);
+          }
+          ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+          if (!ok) break;
+          if (lane < pages)
+#pragma unroll
+            for (int ch = 0; ch < NCH; ++ch)
+              tma_load_3d(sKV + st * S::KV_TILE + ch * (TT_BN * 128) + lane * page * 128, map, come, ch * 64, walk.kvh, slot0);
+          slot0 = slot1;
+          slot1 = slot2;
         }
+        t0 += nt;
       }
-    } else if (warp == 1) {
-      // -------------------------------------------------------------------- MMA issuer
-      // Per group one step at a time: scores, then (once P is there) the product, then the next step's scores, which may be the next piece's.
-      // The whole warp goes through it with the same values; one lane issues.
+    } else if (warp < 3) {
+      // -------------------------------------------------------------------- MMA issuers
+      // A group's steps: scores, then (once P is there) the product, then the next step's scores, which may be the next piece's. The
+      // whole warp goes through it with the same values; one lane issues. With one query tile each group has an issuer; with two, warp 1 issues
+      // for both in turn, so that one's softmax falls beside the other's products (left to themselves they run in step: 191 us, in turn 148, for
+      // 4 trees of 64 nodes, 32 / 4 heads of 128, over 28,000 keys).
       constexpr uint32_t idesc_s = make_idesc(128, TT_BN, 1, 1, 0, 0);
       constexpr uint32_t idesc_o = make_idesc(128, D, 1, 1, 0, 1);  // A = P in TMEM, B = V read MN-major
       const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, UMMA_SWIZZLE_128B);
       const uint64_t k_desc = make_smem_desc(smem_u32(sKV), 16, 1024, UMMA_SWIZZLE_128B);
       const uint64_t v_desc = make_smem_desc(smem_u32(sKV), TT_BN * 128, 1024, UMMA_SWIZZLE_128B);
-      bool ok = true, more = walk.next(a);
-      uint32_t half0 = 0, piece = 0, p_cnt[2] = {0, 0};
-      int j = 0, second = 0;  // the next scores: tile of the piece, and whether they are the second query tile's
-      struct Step {
-        uint32_t v_half, piece;
-        bool there, first, last, frees;
-      } step[2];
+      bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
         ok = ok && mbar_wait(bar, parity, cta_abort, status, code);
         ok = __all_sync(0xffffffffu, ok);
       };
-      auto scores = [&](int g) {
-        step[g].there = false;
-        if (!more) return;
-        const int nt = walk.nt;
-        const bool rows2 = TILES == 2 && walk.groups == 2;
-        const uint32_t kh = half0 + (j == 0 ? 0 : 2 * j - 1);
-        if (!second) {
-          if (j == 0) wait(q_full, piece & 1, ERR_WAIT_FULL);
-          wait(&full[kh % S::RING], (kh / S::RING) & 1, ERR_WAIT_FULL);
-        }
-        if (!ok) return;
-        tc_fence_after();
-        const uint64_t qd = q_desc + second * (S::Q_TILE >> 4), kd = k_desc + (kh % S::RING) * (S::KV_TILE >> 4);
-        const bool done = !rows2 || second, last = done && j + 1 == nt;
-        if (elect_one()) {
+      struct Group {
+        TtWalk<TILES> walk;
+        uint32_t t0, turn, piece, steps;  // tiles and turns of the pieces before, pieces, products so far
+        int i;                            // the next scores: the group's i-th step of the piece
+        bool more;
+        // the step whose scores are issued
+        uint32_t tile, of_piece;
+        bool there, first, last, rows2;
+      };
+      auto scores = [&](Group& s, int g) {
+        s.there = false;
+        while (s.more) {
+          const int nt = s.walk.nt;
+          const bool rows2 = TILES == 2 && s.walk.groups == 2;
+          const int late = (g ^ s.turn) & 1, n_my = rows2 ? nt : (nt + 1 - late) / 2, j = rows2 ? s.i : late + 2 * s.i;
+          if (s.i < n_my) {
+            const uint32_t t = s.t0 + j, ks = t % S::K_RING;
+            if (s.i == 0) wait(q_full, s.piece & 1, ERR_WAIT_FULL);
+            wait(&full[ks], t / S::K_RING & 1, ERR_WAIT_FULL);
+            if (!ok) return;
+            tc_fence_after();
+            const uint64_t qd = q_desc + (rows2 ? late : 0) * (S::Q_TILE >> 4), kd = k_desc + ks * (S::KV_TILE >> 4);
+            const bool last = s.i + 1 == n_my;
+            if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const int at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-            umma_f16(tmem_base + g * TT_BN, qd + at, kd + at, idesc_s, k != 0 ? 1u : 0u);
+              for (int k = 0; k < D / 16; ++k) {
+                const int at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                umma_f16(tmem_base + g * TT_BN, qd + at, kd + at, idesc_s, k != 0 ? 1u : 0u);
+              }
+              umma_commit(&s_full[g]);
+              umma_commit(&empty[ks]);
+              if (!rows2) mbar_arrive(&empty[ks]);  // (the other group has no part in this tile)
+              if (last) umma_commit(q_empty);
+            }
+            __syncwarp();
+            s.there = true;
+            s.of_piece = s.piece;
+            s.tile = t;
+            s.first = s.i == 0;
+            s.last = last;
+            s.rows2 = rows2;
+            ++s.i;
+            return;
           }
-          umma_commit(&s_full[g]);
-          if (done) umma_commit(&empty[kh % S::RING]);
-          if (last) umma_commit(q_empty);
-        }
-        __syncwarp();
-        step[g].there = true;
-        step[g].piece = piece;
-        step[g].v_half = half0 + (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1);
-        step[g].first = rows2 ? j == 0 : j < 2;
-        step[g].last = rows2 ? j + 1 == nt : j + 2 >= nt;
-        step[g].frees = done;
-        second = !done;
-        if (last) {
-          half0 += 2 * nt;
-          j = 0;
-          ++piece;
-          more = walk.next(a);
-        } else if (done) {
-          ++j;
+          if (n_my == 0) {  // no part in this piece: its queries are free as far as this group is concerned, once they are the ones in place
+            wait(q_full, s.piece & 1, ERR_WAIT_FULL);
+            if (!ok) return;
+            if (elect_one()) mbar_arrive(q_empty);
+            __syncwarp();
+          }
+          s.t0 += nt;
+          s.turn += rows2 ? 2 * nt : nt;
+          s.i = 0;
+          ++s.piece;
+          s.more = s.walk.next(a);
         }
       };
-      auto run = [&](int g) -> bool {
-        if (!ok || !step[g].there) return false;
-        wait(&p_full[g], p_cnt[g]++ & 1, ERR_WAIT_TMEM_EMPTY);
-        wait(&full[step[g].v_half % S::RING], (step[g].v_half / S::RING) & 1, ERR_WAIT_FULL);
-        if (step[g].first) wait(o_empty, (step[g].piece & 1) ^ 1, ERR_WAIT_TMEM_EMPTY);  // (the accumulators of the last piece have been read)
+      auto begin = [&](Group& s, int g) {
+        s = {};
+        s.walk = walk;
+        s.more = s.walk.next(a);
+        scores(s, g);
+      };
+      auto step = [&](Group& s, int g) -> bool {
+        if (!ok || !s.there) return false;
+        wait(&p_full[g], s.steps++ & 1, ERR_WAIT_TMEM_EMPTY);
+        const uint32_t vs = s.tile % S::V_RING;
+        wait(&full[S::K_RING + s.tile % S::V_FULL], s.tile / S::V_FULL & 1, ERR_WAIT_FULL);
+        if (s.first) wait(o_empty, (s.of_piece & 1) ^ 1, ERR_WAIT_TMEM_EMPTY);  // (the accumulators of the last piece have been read)
         if (!ok) return false;
         tc_fence_after();
-        const uint64_t vd = v_desc + (step[g].v_half % S::RING) * (S::KV_TILE >> 4);
-        const bool first = step[g].first;
+        const uint64_t vd = v_desc + (S::K_RING + vs) * (S::KV_TILE >> 4);
+        const uint32_t more_o = s.first ? 0u : 1u;
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < TT_BN / 16; ++k)
-            umma_f16_ts(tmem_base + 2 * TT_BN + g * D, tmem_base + g * TT_BN + k * 8, vd + k * (2048 >> 4), idesc_o, (!first || k != 0) ? 1u : 0u);
-          if (step[g].frees) umma_commit(&empty[step[g].v_half % S::RING]);
-          if (step[g].last) umma_commit(&o_full[g]);
+            umma_f16_ts(tmem_base + 2 * TT_BN + g * D, tmem_base + g * TT_BN + k * 8, vd + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more_o);
+          umma_commit(&empty[S::K_RING + vs]);
+          if (!s.rows2) mbar_arrive(&empty[S::K_RING + vs]);
+          if (s.last) umma_commit(&o_full[g]);
         }
         __syncwarp();
-        scores(g);
+        scores(s, g);
         return ok;
       };
-      scores(0);
-      scores(1);
-      while (run(0) && run(1)) {
-      }
-    } else if (warp == 10) {
-      // -------------------------------------------------------------------- queries and ways up, a piece ahead of the others
-      bool ok = true;
-      for (uint32_t piece = 0; ok && walk.next(a); ++piece) {
-        const uint32_t buf = piece & 1;
-        ok = __all_sync(0xffffffffu, mbar_wait(&w_empty[buf], ((piece >> 1) & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY));
-        if (!ok) break;
-        if ((walk.tile0 + walk.nt) * TT_BN > walk.r.ctx) {  // the piece has keys of nodes
-#pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (x * 32 + lane < walk.r.n) par[x * 32 + lane] = a.parents[walk.r.first + x * 32 + lane];
-          __syncwarp();
-          for (int i = lane; i < walk.r.n; i += 32) {
-            uint32_t set[4];
-            tree_way_up([&](int j) { return par[j]; }, i, set);
-            ways[buf * 128 + i] = make_uint4(set[0], set[1], set[2], set[3]);
-          }
-          __syncwarp();
+      if constexpr (TILES == 1) {
+        Group s;
+        begin(s, warp - 1);
+        while (step(s, warp - 1)) {
         }
-        if (lane == 0) {
-          mbar_arrive(&w_full[buf]);
-          ok = mbar_wait(q_empty, (piece & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
-          if (ok) {
-            mbar_arrive_expect_tx(q_full, (REP > 1 ? REP : walk.groups) * a.bq * a.G * 128 * NCH);
-            const int row0 = walk.r.first + walk.pair * TILES * a.bq;
-            // two query tiles, or copies of one
-            for (int x = 0; x < (REP > 1 ? REP : walk.groups); ++x)
-#pragma unroll
-              for (int ch = 0; ch < NCH; ++ch)
-                tma_load_3d(sQ + x * (REP > 1 ? ROWS * 128 : S::Q_TILE) + ch * (128 * 128), &tmQ, q_full, ch * 64, walk.kvh * a.G,
-                            row0 + (REP > 1 ? 0 : x * a.bq));
-          }
+      } else if (warp == 1) {
+        Group s0, s1;
+        begin(s0, 0);
+        begin(s1, 1);
+        while (step(s0, 0) && step(s1, 1)) {
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
     } else {
       // -------------------------------------------------------------------- softmax + epilogue
-      const int quarter = warp & 3, g = (warp - 2) >> 2;
+      const int quarter = warp & 3, g = (warp - 4) >> 2;
       const int row = quarter * 32 + lane;  // row of the query tile = TMEM lane
-      const int tid = (threadIdx.x - 64) & 127;
+      const int tid = threadIdx.x & 127;
       const int copy = row / ROWS, rr = row % ROWS;  // this thread's keys of a tile: columns [copy * COLS, copy * COLS + COLS)
       const int in_tile = rr / a.G, head_in = rr - in_tile * a.G;
+      const int o_rr = tid / REP, o_in = o_rr / a.G, o_head = o_rr - o_in * a.G;  // the row that this thread adds up the copies of
       const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t s_addr = lane_addr + g * TT_BN, o_addr = lane_addr + 2 * TT_BN;
       const uint64_t c2 = f2_pack(a.c_log2, a.c_log2);
-      uint32_t half0 = 0, s_cnt = 0, turn = 0, o_cnt[2] = {0, 0};
+      uint32_t t0 = 0, turn = 0, s_cnt = 0, o_cnt[2] = {0, 0};
       bool ok = true;
       for (uint32_t piece = 0; walk.next(a); ++piece) {  // after an expired wait the threads still meet at the barriers
         const int nt = walk.nt, ctx = walk.r.ctx;
@@ -440,7 +474,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (!have_ways) ok = __all_sync(0xffffffffu, ok && mbar_wait(&w_full[piece & 1], (piece >> 1) & 1, cta_abort, status, ERR_WAIT_FULL));
           have_ways = true;
         };
-        const int n_late = rows2 ? nt : nt / 2;  // steps of the group whose turn is second; the other one has some always
+        const int n_late = rows2 ? nt : nt / 2;  // its steps; the other one has some always
         const int n_my = rows2 ? nt : (late ? n_late : nt - n_late);
         float m_run = -INFINITY, l_run = 0.f;
         for (int i = 0; i < n_my && ok; ++i) {
@@ -557,13 +591,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             f2_unpack(f2_add(sum[0], sum[1]), s0, s1);
             l_run += s0 + s1;
           }
-          if (ends && j + 1 == nt && qt == 0 && (walk.keys & (page - 1)) != 0) {
-            // value rows behind the last key: the rest of its page is cleared (0 x NaN would reach O)
-            const uint32_t h = half0 + 2 * nt - 1;
-            ok = __all_sync(0xffffffffu, mbar_wait(&full[h % S::RING], (h / S::RING) & 1, cta_abort, status, ERR_WAIT_FULL));
+          if (ends && j + 1 == nt && (walk.keys & (page - 1)) != 0) {
+            // value rows behind the last key: the rest of its page is cleared (0 x NaN would reach O), by each group that uses the tile
+            const uint32_t t = t0 + j, vs = S::K_RING + t % S::V_RING;
+            ok = __all_sync(0xffffffffu, mbar_wait(&full[S::K_RING + t % S::V_FULL], t / S::V_FULL & 1, cta_abort, status, ERR_WAIT_FULL));
             if (!ok) break;
             const int from = walk.keys & (TT_BN - 1), to = (from + page - 1) & -page;
-            uint8_t* v = sKV + (h % S::RING) * S::KV_TILE;
+            uint8_t* v = sKV + vs * S::KV_TILE;
             for (int x = tid; x < (to - from) * NCH * 8; x += 128) {
               const int vr = from + x / (NCH * 8), ch = (x / 8) % NCH;
               *reinterpret_cast<uint4*>(v + ch * (TT_BN * 128) + vr * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -659,7 +693,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           // the copies' sums meet in shared memory, 16 columns a turn
           float* mine_red = red + g * (128 * 20);
           constexpr int PER = 16 / REP;  // columns that a thread adds up, of row tid / REP
-          const int o_rr = tid / REP, o_in = o_rr / a.G;
           const bool o_valid = o_in < walk.r.n && o_in < a.bq;
 #pragma unroll 1
           for (int col = g * (D / 2); col < (g + 1) * (D / 2); col += 16) {
@@ -690,7 +723,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                 }
               const int at = col + (tid % REP) * PER;
               if (all) {
-                __nv_bfloat16* dst = a.out + static_cast<long>(walk.r.first + o_in) * a.out_row + static_cast<long>(walk.kvh * a.G + o_rr - o_in * a.G) * D + at;
+                __nv_bfloat16* dst = a.out + static_cast<long>(walk.r.first + o_in) * a.out_row + static_cast<long>(walk.kvh * a.G + o_head) * D + at;
 #pragma unroll
                 for (int k = 0; k < PER; k += 4)
                   *reinterpret_cast<uint2*>(dst + k) = make_uint2(pack_bf16x2(t[k], t[k + 1]), pack_bf16x2(t[k + 2], t[k + 3]));
@@ -709,7 +742,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(o_empty);
-        half0 += 2 * nt;
+        t0 += nt;
         turn += rows2 ? 2 * nt : nt;
       }
     }
