@@ -341,6 +341,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       // 4 trees of 64 nodes, 32 / 4 heads of 128, over 28,000 keys).
       constexpr uint32_t idesc_s = make_idesc(128, TT_BN, 1, 1, 0, 0);
       constexpr uint32_t idesc_o = make_idesc(128, D, 1, 1, 0, 1);  // A = P in TMEM, B = V read MN-major
+      // operands of the products come from registers that are the same for the whole warp: without the compiler knowing it each product costs some 100 cycles
+      auto uniform = [](uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); };
+      const uint32_t tmem = uniform(tmem_base);
       const uint64_t q_desc = make_smem_desc(smem_u32(sQ), 16, 1024, UMMA_SWIZZLE_128B);
       const uint64_t k_desc = make_smem_desc(smem_u32(sKV), 16, 1024, UMMA_SWIZZLE_128B);
       const uint64_t v_desc = make_smem_desc(smem_u32(sKV), TT_BN * 128, 1024, UMMA_SWIZZLE_128B);
@@ -370,13 +373,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             wait(&full[ks], t / S::K_RING & 1, ERR_WAIT_FULL);
             if (!ok) return;
             tc_fence_after();
-            const uint64_t qd = q_desc + (rows2 ? late : 0) * (S::Q_TILE >> 4), kd = k_desc + ks * (S::KV_TILE >> 4);
+            const uint64_t qd = q_desc + uniform(rows2 ? late : 0) * (S::Q_TILE >> 4), kd = k_desc + uniform(ks) * (S::KV_TILE >> 4);
+            const uint32_t d_s = tmem + uniform(g) * TT_BN;
             const bool last = s.i + 1 == n_my;
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < D / 16; ++k) {
                 const int at = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
-                umma_f16(tmem_base + g * TT_BN, qd + at, kd + at, idesc_s, k != 0 ? 1u : 0u);
+                umma_f16(d_s, qd + at, kd + at, idesc_s, k != 0 ? 1u : 0u);
               }
               umma_commit(&s_full[g]);
               umma_commit(&empty[ks]);
@@ -420,12 +424,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         if (s.first) wait(o_empty, (s.of_piece & 1) ^ 1, ERR_WAIT_TMEM_EMPTY);  // (the accumulators of the last piece have been read)
         if (!ok) return false;
         tc_fence_after();
-        const uint64_t vd = v_desc + (S::K_RING + vs) * (S::KV_TILE >> 4);
-        const uint32_t more_o = s.first ? 0u : 1u;
+        const uint64_t vd = v_desc + (S::K_RING + uniform(vs)) * (S::KV_TILE >> 4);
+        const uint32_t more_o = uniform(s.first ? 0u : 1u), d_o = tmem + 2 * TT_BN + uniform(g) * D, a_o = tmem + uniform(g) * TT_BN;
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < TT_BN / 16; ++k)
-            umma_f16_ts(tmem_base + 2 * TT_BN + g * D, tmem_base + g * TT_BN + k * 8, vd + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more_o);
+            umma_f16_ts(d_o, a_o + k * 8, vd + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more_o);
           umma_commit(&empty[S::K_RING + vs]);
           if (!s.rows2) mbar_arrive(&empty[S::K_RING + vs]);
           if (s.last) umma_commit(&o_full[g]);
@@ -457,7 +461,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t s_addr = lane_addr + g * TT_BN, o_addr = lane_addr + 2 * TT_BN;
       const uint64_t c2 = f2_pack(a.c_log2, a.c_log2);
-      uint32_t t0 = 0, turn = 0, s_cnt = 0, o_cnt[2] = {0, 0};
+      uint32_t t0 = 0, turn = 0, s_cnt = 0, o_cnt0 = 0, o_cnt1 = 0;
       bool ok = true;
       for (uint32_t piece = 0; walk.next(a); ++piece) {  // after an expired wait the threads still meet at the barriers
         const int nt = walk.nt, ctx = walk.r.ctx;
@@ -621,7 +625,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const bool all = walk.tile0 == 0 && ends;
         const int slot = 2 * c + (piece == 0 ? 0 : 1);
         const int g_first = turn & 1;  // the group whose turn was first
-        const bool has[2] = {g_first == 0 || n_late > 0, g_first == 1 || n_late > 0};
+        const bool has0 = g_first == 0 || n_late > 0, has1 = g_first == 1 || n_late > 0;
         float f0 = 1.f, f1 = 0.f, m = m_run, l = l_run;
         if (!rows2) {
           float2* mine_ml = ml + (piece & 1) * 256;
@@ -642,12 +646,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
           }
         }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (has[x] && (!rows2 || x == g)) ok = ok && mbar_wait(&o_full[x], o_cnt[x] & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
+        if (has0 && (!rows2 || g == 0)) ok = ok && mbar_wait(&o_full[0], o_cnt0 & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
+        if (has1 && (!rows2 || g == 1)) ok = ok && mbar_wait(&o_full[1], o_cnt1 & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
         ok = __all_sync(0xffffffffu, ok);
-        o_cnt[0] += has[0];
-        o_cnt[1] += has[1];
+        o_cnt0 += has0;
+        o_cnt1 += has1;
         tc_fence_after();
         float inv = 1.f;
         if (all) {
@@ -655,45 +658,50 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (a.sinks != nullptr && valid && l > 0.f) l += tt_exp2(a.sinks[head] * 1.4426950408889634f - m);
           inv = (l > 0.f && !hole) ? 1.f / l : 0.f;
         }
-        // 8 columns of row `r` of the tile: to the output, or as this part's sums
-        auto put = [&](int r, int node_, int head_, int col, const float (&x)[8], float by) {
-          if (all) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (by > 0.f) v = make_uint4(pack_bf16x2(x[0] * by, x[1] * by), pack_bf16x2(x[2] * by, x[3] * by), pack_bf16x2(x[4] * by, x[5] * by), pack_bf16x2(x[6] * by, x[7] * by));
-            *reinterpret_cast<uint4*>(a.out + static_cast<long>(walk.r.first + node_) * a.out_row + static_cast<long>(walk.kvh * a.G + head_) * D + col) = v;
-          } else {
-            float4* p = reinterpret_cast<float4*>(a.part_o + (static_cast<long>(slot) * (128 * TILES) + r) * D + col);
-            p[0] = make_float4(x[0], x[1], x[2], x[3]);
-            p[1] = make_float4(x[4], x[5], x[6], x[7]);
-          }
-        };
+        // an accumulator that nothing was added to holds anything, and a row that sees nothing is zero whatever its accumulators hold
+        const float by0 = f0 * inv, by1 = f1 * inv;
+        const uint32_t keep0 = has0 && by0 > 0.f ? 0xffffffffu : 0u, keep1 = has1 && by1 > 0.f ? 0xffffffffu : 0u;
+        auto both = [&](uint32_t x, uint32_t y) { return fmaf(__uint_as_float(x & keep0), by0, __uint_as_float(y & keep1) * by1); };
         if constexpr (REP == 1) {
           if (ok && active) {
+            // a thread writes its row: all of it, or half
             const int col0 = rows2 ? 0 : g * (D / 2), cols = rows2 ? D : D / 2;
+            __nv_bfloat16* o_row = a.out + static_cast<long>(walk.r.first + node) * a.out_row + static_cast<long>(walk.kvh * a.G + head_in) * D;
+            float* p_row = a.part_o + (static_cast<long>(slot) * (128 * TILES) + qt * 128 + row) * D;
+            const uint32_t mine_o = o_addr + (rows2 ? g * D : 0);
 #pragma unroll 1
             for (int col = col0; col < col0 + cols; col += 16) {
               uint32_t x[16], y[16];
-              tmem_ld_32x16(o_addr + (rows2 ? g * D : 0) + col, x);
+              tmem_ld_32x16(mine_o + col, x);
               if (!rows2) tmem_ld_32x16(o_addr + D + col, y);
               tmem_ld_wait();
               float v[16];
+              if (rows2) {
 #pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                // (an accumulator that nothing was added to holds anything)
-                v[k] = rows2 ? __uint_as_float(x[k]) : (has[0] ? __uint_as_float(x[k]) * f0 : 0.f) + (has[1] ? __uint_as_float(y[k]) * f1 : 0.f);
+                for (int k = 0; k < 16; ++k) v[k] = inv > 0.f ? __uint_as_float(x[k]) * inv : 0.f;
+              } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = both(x[k], y[k]);
               }
-              if (valid) {
-                const float lo[8] = {v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}, hi[8] = {v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]};
-                put(qt * 128 + row, node, head_in, col, lo, inv);
-                put(qt * 128 + row, node, head_in, col + 8, hi, inv);
+              if (valid && all) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 8)
+                  *reinterpret_cast<uint4*>(o_row + col + k) = make_uint4(pack_bf16x2(v[k], v[k + 1]), pack_bf16x2(v[k + 2], v[k + 3]),
+                                                                          pack_bf16x2(v[k + 4], v[k + 5]), pack_bf16x2(v[k + 6], v[k + 7]));
+              } else if (valid) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(p_row + col + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
               }
             }
           }
         } else {
-          // the copies' sums meet in shared memory, 16 columns a turn
+          // the copies' sums meet in shared memory, 16 columns a turn; then a thread adds up 16 / REP columns of row tid / REP
           float* mine_red = red + g * (128 * 20);
-          constexpr int PER = 16 / REP;  // columns that a thread adds up, of row tid / REP
-          const bool o_valid = o_in < walk.r.n && o_in < a.bq;
+          constexpr int PER = 16 / REP;
+          const bool o_valid = ok && o_in < walk.r.n && o_in < a.bq;
+          __nv_bfloat16* o_row = a.out + static_cast<long>(walk.r.first + o_in) * a.out_row + static_cast<long>(walk.kvh * a.G + o_head) * D + (tid % REP) * PER;
+          float* p_row = a.part_o + (static_cast<long>(slot) * 128 + o_rr) * D + (tid % REP) * PER;
+          const float* from = mine_red + o_rr * 20 + (tid % REP) * PER;
 #pragma unroll 1
           for (int col = g * (D / 2); col < (g + 1) * (D / 2); col += 16) {
             if (ok && active) {
@@ -701,16 +709,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               tmem_ld_32x16(o_addr + col, x);
               tmem_ld_32x16(o_addr + D + col, y);
               tmem_ld_wait();
-              float v[16];
-#pragma unroll
-              for (int k = 0; k < 16; ++k)
-                v[k] = inv > 0.f ? ((has[0] ? __uint_as_float(x[k]) * f0 : 0.f) + (has[1] ? __uint_as_float(y[k]) * f1 : 0.f)) * inv : 0.f;
 #pragma unroll
               for (int k = 0; k < 16; k += 4)
-                *reinterpret_cast<float4*>(mine_red + row * 20 + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                *reinterpret_cast<float4*>(mine_red + row * 20 + k) = make_float4(both(x[k], y[k]), both(x[k + 1], y[k + 1]), both(x[k + 2], y[k + 2]),
+                                                                                  both(x[k + 3], y[k + 3]));
             }
             tt_barrier(1 + g, 128);
-            if (o_valid && ok) {
+            if (o_valid) {
               float t[PER];
 #pragma unroll
               for (int k = 0; k < PER; ++k) t[k] = 0.f;
@@ -718,19 +723,13 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               for (int x = 0; x < REP; ++x)
 #pragma unroll
                 for (int k = 0; k < PER; k += 4) {
-                  const float4 e = *reinterpret_cast<const float4*>(mine_red + (x * ROWS + o_rr) * 20 + (tid % REP) * PER + k);
+                  const float4 e = *reinterpret_cast<const float4*>(from + x * (ROWS * 20) + k);
                   t[k] += e.x; t[k + 1] += e.y; t[k + 2] += e.z; t[k + 3] += e.w;
                 }
-              const int at = col + (tid % REP) * PER;
-              if (all) {
-                __nv_bfloat16* dst = a.out + static_cast<long>(walk.r.first + o_in) * a.out_row + static_cast<long>(walk.kvh * a.G + o_head) * D + at;
 #pragma unroll
-                for (int k = 0; k < PER; k += 4)
-                  *reinterpret_cast<uint2*>(dst + k) = make_uint2(pack_bf16x2(t[k], t[k + 1]), pack_bf16x2(t[k + 2], t[k + 3]));
-              } else {
-                float* dst = a.part_o + (static_cast<long>(slot) * 128 + o_rr) * D + at;
-#pragma unroll
-                for (int k = 0; k < PER; k += 4) *reinterpret_cast<float4*>(dst + k) = make_float4(t[k], t[k + 1], t[k + 2], t[k + 3]);
+              for (int k = 0; k < PER; k += 4) {
+                if (all) *reinterpret_cast<uint2*>(o_row + col + k) = make_uint2(pack_bf16x2(t[k], t[k + 1]), pack_bf16x2(t[k + 2], t[k + 3]));
+                else *reinterpret_cast<float4*>(p_row + col + k) = make_float4(t[k], t[k + 1], t[k + 2], t[k + 3]);
               }
             }
             tt_barrier(1 + g, 128);
