@@ -24,7 +24,7 @@
 //
 // Key and value tiles have a ring of buffers each, with a producer of its own, and the rings run on from one piece of work to the next. Every
 // waiter sees every phase of a barrier: a wait by parity cannot tell one phase from the next but one. Even rings give that to the groups, which
-// take tiles in turn; a ring of three buffers has six barriers for it; with two query tiles one warp waits for both groups. The scores of hidden nodes become -infinity by a bit mask per row, looked at in the last tiles only. Cache rows behind
+// take tiles in turn; a ring of three buffers has six barriers for it. The scores of hidden nodes become -infinity by a bit mask per row, looked at in the last tiles only. Cache rows behind
 // the last node may hold anything: pages behind it are fetched from outside the cache, which reads as zero, and the rest of its page is
 // cleared in shared memory before the product of weights (zero) and values.
 // Every wait is bounded: on expiry the CTA records a status word, drains and returns with its TMEM freed.
@@ -56,6 +56,13 @@ __device__ __forceinline__ float tt_exp2(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// mbar_wait (common.cuh) with everything behind the first few looks out of line: a step's code has to stay small, see the top of this file.
+__device__ __noinline__ bool tt_wait_long(uint64_t* bar, uint32_t parity, volatile int* cta_abort, int* status, int code) {
+  return mbar_wait(bar, parity, cta_abort, status, code);
+}
+__device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t parity, volatile int* cta_abort, int* status, int code) {
+  return mbar_try_wait(bar, parity) || tt_wait_long(bar, parity, cta_abort, status, code);
 }
 __device__ __forceinline__ void tt_barrier(int id, int nthreads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory"); }
 
@@ -161,7 +168,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* o_empty = o_full + 2;      // both accumulators have been read (8 arrivals)
   uint64_t* w_full = o_empty + 1;      // [2] ways of the piece are there
   uint64_t* w_empty = w_full + 2;      // [2] ... and have been used (8 arrivals)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(w_empty + 2);
+  uint64_t* my_turn = w_empty + 2;     // [2] the other group's issuer is done with its step
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(my_turn + 2);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 2);  // [0] request, [1] unit within it
   int* sums = start + 2;                               // [12] units of the warps' requests
@@ -179,6 +187,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       mbar_init(&o_full[g], 1);
       mbar_init(&w_full[g], 1);
       mbar_init(&w_empty[g], 8);
+      mbar_init(&my_turn[g], 1);
     }
     mbar_init(o_empty, 8);
     *cta_abort = 0;
@@ -280,7 +289,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           }
         } else {
           const uint32_t buf = piece & 1;
-          ok = __all_sync(0xffffffffu, mbar_wait(&w_empty[buf], ((piece >> 1) & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY));
+          ok = __all_sync(0xffffffffu, tt_wait(&w_empty[buf], ((piece >> 1) & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY));
           if (!ok) break;
           const bool hides = (walk.tile0 + nt) * TT_BN > walk.r.ctx;  // the piece has keys of nodes
           if (hides) {
@@ -289,7 +298,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               if (x * 32 + lane < walk.r.n) par[x * 32 + lane] = a.parents[walk.r.first + x * 32 + lane];
           }
           if (lane == 0) {
-            ok = mbar_wait(q_empty, (piece & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
+            ok = tt_wait(q_empty, (piece & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
             if (ok) {
               mbar_arrive_expect_tx(q_full, (REP > 1 ? REP : walk.groups) * a.bq * a.G * 128 * NCH);
               const int row0 = walk.r.first + walk.pair * TILES * a.bq;
@@ -319,7 +328,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           const uint32_t ring = is_k ? S::K_RING : S::V_RING, t = t0 + j, st = t % ring + (is_k ? 0 : S::K_RING);
           uint64_t* come = &full[is_k ? st : S::K_RING + t % S::V_FULL];
           if (lane == 0) {
-            ok = mbar_wait(&empty[st], (t / ring & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
+            ok = tt_wait(&empty[st], (t / ring & 1) ^ 1, cta_abort, status, ERR_WAIT_EMPTY);
             if (ok) mbar_arrive_expect_tx(come, S::KV_TILE);
           }
           ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -336,9 +345,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     } else if (warp < 3) {
       // -------------------------------------------------------------------- MMA issuers
       // A group's steps: scores, then (once P is there) the product, then the next step's scores, which may be the next piece's. The
-      // whole warp goes through it with the same values; one lane issues. With one query tile each group has an issuer; with two, warp 1 issues
-      // for both in turn, so that one's softmax falls beside the other's products (left to themselves they run in step: 191 us, in turn 148, for
-      // 4 trees of 64 nodes, 32 / 4 heads of 128, over 28,000 keys).
+      // whole warp goes through it with the same values; one lane issues. With two query tiles the issuers take turns, so that one group's
+      // softmax falls beside the other's products (left to themselves they run in step: 191 us, in turn 152, for 4 trees of 64 nodes, 32 / 4
+      // heads of 128, over 28,000 keys).
       constexpr uint32_t idesc_s = make_idesc(128, TT_BN, 1, 1, 0, 0);
       constexpr uint32_t idesc_o = make_idesc(128, D, 1, 1, 0, 1);  // A = P in TMEM, B = V read MN-major
       // operands of the products come from registers that are the same for the whole warp: without the compiler knowing it each product costs some 100 cycles
@@ -349,7 +358,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const uint64_t v_desc = make_smem_desc(smem_u32(sKV), TT_BN * 128, 1024, UMMA_SWIZZLE_128B);
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-        ok = ok && mbar_wait(bar, parity, cta_abort, status, code);
+        ok = ok && tt_wait(bar, parity, cta_abort, status, code);
         ok = __all_sync(0xffffffffu, ok);
       };
       struct Group {
@@ -422,6 +431,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const uint32_t vs = s.tile % S::V_RING;
         wait(&full[S::K_RING + s.tile % S::V_FULL], s.tile / S::V_FULL & 1, ERR_WAIT_FULL);
         if (s.first) wait(o_empty, (s.of_piece & 1) ^ 1, ERR_WAIT_TMEM_EMPTY);  // (the accumulators of the last piece have been read)
+        if (TILES == 2) wait(&my_turn[g], (s.steps - 1) & 1, ERR_WAIT_EMPTY);
         if (!ok) return false;
         tc_fence_after();
         const uint64_t vd = v_desc + (S::K_RING + uniform(vs)) * (S::KV_TILE >> 4);
@@ -436,19 +446,16 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         }
         __syncwarp();
         scores(s, g);
+        if (TILES == 2 && elect_one()) mbar_arrive(&my_turn[g ^ 1]);
+        __syncwarp();
         return ok;
       };
-      if constexpr (TILES == 1) {
-        Group s;
-        begin(s, warp - 1);
-        while (step(s, warp - 1)) {
-        }
-      } else if (warp == 1) {
-        Group s0, s1;
-        begin(s0, 0);
-        begin(s1, 1);
-        while (step(s0, 0) && step(s1, 1)) {
-        }
+      const int g = warp - 1;
+      if (TILES == 2 && g == 1 && elect_one()) mbar_arrive(&my_turn[0]);  // group 0 begins
+      __syncwarp();
+      Group s;
+      begin(s, g);
+      while (step(s, g)) {
       }
     } else {
       // -------------------------------------------------------------------- softmax + epilogue
@@ -475,7 +482,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         const uint32_t* way = reinterpret_cast<const uint32_t*>(&ways[(piece & 1) * 128 + (valid ? node : 0)]);
         bool have_ways = false;
         auto want_ways = [&]() {
-          if (!have_ways) ok = __all_sync(0xffffffffu, ok && mbar_wait(&w_full[piece & 1], (piece >> 1) & 1, cta_abort, status, ERR_WAIT_FULL));
+          if (!have_ways) ok = __all_sync(0xffffffffu, ok && tt_wait(&w_full[piece & 1], (piece >> 1) & 1, cta_abort, status, ERR_WAIT_FULL));
           have_ways = true;
         };
         const int n_late = rows2 ? nt : nt / 2;  // its steps; the other one has some always
@@ -483,7 +490,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         float m_run = -INFINITY, l_run = 0.f;
         for (int i = 0; i < n_my && ok; ++i) {
           const int j = rows2 ? i : late + 2 * i;
-          ok = mbar_wait(&s_full[g], (s_cnt + i) & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
+          ok = tt_wait(&s_full[g], (s_cnt + i) & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
@@ -514,30 +521,23 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               }
               return fmaxf(m0, m1);
             };
-            // A row of 128 columns is read twice, in quarters: for its maximum the last two, then the first two, which stay in
-            // registers; the last two come back behind those (P takes the columns of the first two only).
+            // A row of 128 columns is read twice: for its maximum the second half, then the first one, which stays in registers; the second half
+            // comes back behind that (P takes the columns of the first half only).
             uint32_t ra[32], rb[32];
             float mx = -INFINITY;
             const int x0 = copy * (COLS / 32);
-            if constexpr (COLS == 128) {
-              tmem_ld_32x32(s_addr + 64, ra);
-              tmem_ld_32x32(s_addr + 96, rb);
+#pragma unroll 1
+            for (int x = x0 + (COLS == 128 ? 2 : 0); x >= x0; x -= 2) {
+              tmem_ld_32x32(s_addr + 32 * x, ra);
+              if constexpr (COLS > 32) tmem_ld_32x32(s_addr + 32 * x + 32, rb);
               tmem_ld_wait();
               if (masked) {
-                hide(ra, 2);
-                hide(rb, 3);
+                hide(ra, x);
+                if constexpr (COLS > 32) hide(rb, x + 1);
               }
-              mx = fmaxf(top(ra), top(rb));
+              mx = fmaxf(mx, COLS > 32 ? fmaxf(top(ra), top(rb)) : top(ra));
             }
-            tmem_ld_32x32(s_addr + 32 * x0, ra);
-            if constexpr (COLS > 32) tmem_ld_32x32(s_addr + 32 * x0 + 32, rb);
-            tmem_ld_wait();
-            if (masked) {
-              hide(ra, x0);
-              if constexpr (COLS > 32) hide(rb, x0 + 1);
-            }
-            const float m01 = COLS > 32 ? fmaxf(top(ra), top(rb)) : top(ra);
-            mx = fmaxf(mx, m01) * a.c_log2;  // c > 0: the maximum commutes with the scaling
+            mx *= a.c_log2;  // c > 0: the maximum commutes with the scaling
             const float m_new = fmaxf(m_run, mx);
             if (i == 0) {
               m_run = m_new;
@@ -579,17 +579,19 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               for (int x = 0; x < 4; ++x)
                 if (x < x0 || x >= x0 + COLS / 32) tmem_st_32x16(s_addr + x * 16, none);
             }
-            weigh(ra, x0);
-            if constexpr (COLS == 128) tmem_ld_32x32(s_addr + 64, ra);
-            if constexpr (COLS > 32) weigh(rb, x0 + 1);
-            if constexpr (COLS == 128) {
-              tmem_ld_wait();
-              tmem_ld_32x32(s_addr + 96, rb);
-              if (masked) hide(ra, 2);
-              weigh(ra, 2);
-              tmem_ld_wait();
-              if (masked) hide(rb, 3);
-              weigh(rb, 3);
+#pragma unroll 1
+            for (int x = x0; x < x0 + (COLS + 63) / 64 * 2; x += 2) {
+              if (COLS == 128 && x > x0) {
+                tmem_ld_32x32(s_addr + 32 * x, ra);
+                tmem_ld_32x32(s_addr + 32 * x + 32, rb);
+                tmem_ld_wait();
+                if (masked) {
+                  hide(ra, x);
+                  hide(rb, x + 1);
+                }
+              }
+              weigh(ra, x);
+              if constexpr (COLS > 32) weigh(rb, x + 1);
             }
             float s0, s1;
             f2_unpack(f2_add(sum[0], sum[1]), s0, s1);
@@ -598,7 +600,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (ends && j + 1 == nt && (walk.keys & (page - 1)) != 0) {
             // value rows behind the last key: the rest of its page is cleared (0 x NaN would reach O), by each group that uses the tile
             const uint32_t t = t0 + j, vs = S::K_RING + t % S::V_RING;
-            ok = __all_sync(0xffffffffu, mbar_wait(&full[S::K_RING + t % S::V_FULL], t / S::V_FULL & 1, cta_abort, status, ERR_WAIT_FULL));
+            ok = __all_sync(0xffffffffu, tt_wait(&full[S::K_RING + t % S::V_FULL], t / S::V_FULL & 1, cta_abort, status, ERR_WAIT_FULL));
             if (!ok) break;
             const int from = walk.keys & (TT_BN - 1), to = (from + page - 1) & -page;
             uint8_t* v = sKV + vs * S::KV_TILE;
@@ -646,8 +648,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             }
           }
         }
-        if (has0 && (!rows2 || g == 0)) ok = ok && mbar_wait(&o_full[0], o_cnt0 & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
-        if (has1 && (!rows2 || g == 1)) ok = ok && mbar_wait(&o_full[1], o_cnt1 & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
+        if (has0 && (!rows2 || g == 0)) ok = ok && tt_wait(&o_full[0], o_cnt0 & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
+        if (has1 && (!rows2 || g == 1)) ok = ok && tt_wait(&o_full[1], o_cnt1 & 1, cta_abort, status, ERR_WAIT_TMEM_FULL);
         ok = __all_sync(0xffffffffu, ok);
         o_cnt0 += has0;
         o_cnt1 += has1;
