@@ -148,19 +148,28 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
 
 }  // namespace sb
 
-// in / out: [rows, vocab] of pitch in_row / out_row elements, bf16 or fp32 alike; they may be the same. Tokens outside the vocabulary
-// (of texts, trees and biases) count for nothing. With trees, row r is node r - cu[b] of tree b; rows behind cu[requests] are left as they are.
-extern "C" int sb_adjust_logits(const void* in, void* out, const int* tokens, const int* lengths, const int* prompts, const float* repetition,
-                                const float* frequency, const float* presence, const int* bias_ids, const float* bias_values,
-                                const int* allowed, const int* drafted, const int* parents, const int* cu, long in_row, long out_row,
-                                long tokens_row, long bias_row, long allowed_row, int rows, int requests, int vocab, int text, int biases,
-                                int f32, cudaStream_t s) {
-  if (rows <= 0 || vocab <= 0) return 0;
-  const sb::LogitsArgs a = {in, out, tokens, lengths, prompts, repetition, frequency, presence, bias_ids, bias_values, allowed, drafted, parents,
-                            cu, in_row, out_row, tokens_row, bias_row, allowed_row, rows, requests, vocab, text, biases};
+// call: addresses of in, out, tokens, lengths, prompts, repetition, frequency, presence, bias ids, bias values, allowed, drafted, parents, cu (null: not there); then
+// the pitches of in, out, tokens, biases and allowed (elements), rows, requests, vocabulary, tokens of a text, biases of a request, whether in and
+// out are fp32 (else bf16). in and out may be the same. Tokens outside the vocabulary (of texts, trees and biases) count for nothing. With trees, row r is
+// node r - cu[b] of tree b; rows behind cu[requests] are left as they are.
+extern "C" int sb_adjust_logits(const void* call, cudaStream_t s) {
+  const long long* x = static_cast<const long long*>(call);
+  auto ints = [&](int i) { return reinterpret_cast<const int*>(x[i]); };
+  auto floats = [&](int i) { return reinterpret_cast<const float*>(x[i]); };
+  sb::LogitsArgs a = {};
+  a.in = reinterpret_cast<const void*>(x[0]);
+  a.out = reinterpret_cast<void*>(x[1]);
+  a.tokens = ints(2); a.lengths = ints(3); a.prompts = ints(4);
+  a.repetition = floats(5); a.frequency = floats(6); a.presence = floats(7);
+  a.bias_ids = ints(8); a.bias_values = floats(9);
+  a.allowed = ints(10);
+  a.drafted = ints(11); a.parents = ints(12); a.cu = ints(13);
+  a.in_row = x[14]; a.out_row = x[15]; a.tokens_row = x[16]; a.bias_row = x[17]; a.allowed_row = x[18];
+  a.rows = x[19]; a.requests = x[20]; a.vocab = x[21]; a.text = x[22]; a.biases = x[23];
+  if (a.rows <= 0 || a.vocab <= 0) return 0;
   const dim3 block(sb::LG_THREADS);
-  const long ctas = (static_cast<long>(vocab) + sb::LG_CHUNK - 1) / sb::LG_CHUNK * rows;
+  const long ctas = (static_cast<long>(a.vocab) + sb::LG_CHUNK - 1) / sb::LG_CHUNK * a.rows;
   if (ctas > 0x7fffffffl) return (int)cudaErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(ctas));
-  return (int)(f32 ? sb::launch_pdl(sb::logits_kernel<float>, grid, block, 0, s, a) : sb::launch_pdl(sb::logits_kernel<__nv_bfloat16>, grid, block, 0, s, a));
+  return (int)(x[24] ? sb::launch_pdl(sb::logits_kernel<float>, grid, block, 0, s, a) : sb::launch_pdl(sb::logits_kernel<__nv_bfloat16>, grid, block, 0, s, a));
 }

@@ -127,28 +127,28 @@ tree_accept_kernel(const int* __restrict__ sampled, const int* __restrict__ draf
 
 }  // namespace sb
 
-// path, tokens: [B, max_nodes], -1 behind the accepted nodes; count: [B] (all three are written when `writes`). bases: n_bases addresses, each the
-// first of `layers` slabs that lie `step` bytes apart; rows of row_units * unit bytes, row_bytes apart. n_bases 0: nothing is moved.
-extern "C" int sb_tree_accept(const int* sampled, const int* drafted, const int* parents, const int* cu, int* path, int* tokens, int* count, int rows, int B,
-                              int max_nodes, const void* bases, int n_bases, int layers, long step, int slots, int row_units, int unit,
-                              long row_bytes, const int* table, const int* context, int page_size, int max_pages, int writes, int sms,
-                              cudaStream_t s) {
+// call: addresses of sampled, drafted, parents, cu, path, tokens, count, page table and context lengths; then rows, B, most nodes, page size, pages of a row
+// of the table, whether to write path, tokens and count, SMs, slabs behind each address, bytes between them, slots, pieces of a row, bytes of a
+// piece (2, 4, 8 or 16), bytes from one slot to the next, number of addresses, and the addresses, each the first of so many slabs. path, tokens:
+// [B, max_nodes], -1 behind the accepted nodes; count: [B]. No address: nothing is moved.
+extern "C" int sb_tree_accept(const void* call, cudaStream_t s) {
+  const long long* x = static_cast<const long long*>(call);
+  auto ints = [&](int i) { return reinterpret_cast<int*>(x[i]); };
+  const int rows = x[9], B = x[10], max_nodes = x[11], page_size = x[12], max_pages = x[13], writes = x[14], sms = x[15], layers = x[16], n = x[22];
   if (B <= 0) return 0;
-  if (max_nodes <= 0 || max_nodes > sb::TREE_MAX || n_bases < 0 || n_bases > sb::AC_SLABS || (n_bases > 0 && (page_size <= 0 || layers <= 0)))
-    return (int)cudaErrorInvalidValue;
+  if (max_nodes <= 0 || max_nodes > sb::TREE_MAX || n < 0 || n > sb::AC_SLABS || (n > 0 && (page_size <= 0 || layers <= 0))) return (int)cudaErrorInvalidValue;
   sb::AcceptSlabs c = {};
-  const unsigned long long* from = reinterpret_cast<const unsigned long long*>(bases);
-  for (int i = 0; i < n_bases; ++i) c.base[i] = reinterpret_cast<uint8_t*>(from[i]);
-  c.step = step;
+  for (int i = 0; i < n; ++i) c.base[i] = reinterpret_cast<uint8_t*>(x[23 + i]);
   c.layers = layers;
-  c.count = n_bases * layers;
-  c.slots = slots;
-  c.row_units = row_units;
-  c.unit = unit;
-  c.row_bytes = row_bytes;
-  const long all = (static_cast<long>(c.count) * row_units + sb::AC_THREADS - 1) / sb::AC_THREADS;
+  c.step = x[17];
+  c.count = n * layers;
+  c.slots = static_cast<int>(x[18]);
+  c.row_units = static_cast<int>(x[19]);
+  c.unit = static_cast<int>(x[20]);
+  c.row_bytes = x[21];
+  const long all = (static_cast<long>(c.count) * c.row_units + sb::AC_THREADS - 1) / sb::AC_THREADS;
   const long want = (4L * sms + B - 1) / B;
   const int parts = static_cast<int>(all < 1 ? 1 : (all < want ? all : want));
-  return (int)sb::launch_pdl(sb::tree_accept_kernel, dim3(B, parts), dim3(sb::AC_THREADS), 0, s, sampled, drafted, parents, cu, path, tokens, count,
-                             rows, max_nodes, c, table, context, page_size, max_pages, writes);
+  return (int)sb::launch_pdl(sb::tree_accept_kernel, dim3(B, parts), dim3(sb::AC_THREADS), 0, s, ints(0), ints(1), ints(2), ints(3), ints(4), ints(5), ints(6),
+                             rows, max_nodes, c, ints(7), ints(8), page_size, max_pages, writes);
 }

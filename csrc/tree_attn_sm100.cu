@@ -861,40 +861,45 @@ extern "C" int sb_tree_attn_plan(int B, int Hq, int Hkv, int D, int max_nodes, l
   return 0;
 }
 
-// Arguments as for sb_tree_attn (tree_attn.cu), bf16. scale > 0. work: 16-byte aligned workspace of the size that sb_tree_attn_plan names.
+// call: addresses of q, both caches, page table, context lengths, cu, parents, sinks, out, workspace, status word; then rows, B, Hq, Hkv, D, page size, pages of
+// a row of the table, slots, most nodes, pitches of q (row, head), k (slot, head), v (slot, head) and out (row), whole, bytes of workspace, SMs (one
+// array: a call from Python costs some 0.1 us for every argument). Everything as for sb_tree_attn (tree_attn.cu), in bf16; scale > 0; a
+// 16-byte aligned workspace of the size that sb_tree_attn_plan names.
 // Returns 0, a cudaError_t value, or -1 where this kernel does not cover the call: head widths other than 64 and 128, pages other than
 // 16, 32, 64 and 128 tokens, more than 128 query heads on a key head, addresses or pitches that are no multiple of 16 bytes.
-extern "C" int sb_tree_attn_tc(const void* q, const void* k_cache, const void* v_cache, const int* table, const int* context, const int* cu,
-                               const int* parents, const float* sinks, void* out, int rows, int B, int Hq, int Hkv, int D, int page_size,
-                               int max_pages, int num_slots, int max_nodes, long q_row, long q_head, long k_row, long k_head, long v_row,
-                               long v_head, long out_row, float scale, int whole, void* work, long work_bytes, int sms, int* status,
-                               cudaStream_t s) {
+extern "C" int sb_tree_attn_tc(const void* call, float scale, cudaStream_t s) {
+  const long long* x = static_cast<const long long*>(call);
+  const int rows = x[11], B = x[12], Hq = x[13], Hkv = x[14], D = x[15], page_size = x[16], max_pages = x[17], num_slots = x[18], max_nodes = x[19];
+  const long q_row = x[20], q_head = x[21], k_row = x[22], k_head = x[23], v_row = x[24], v_head = x[25], out_row = x[26];
+  const int whole = x[27], sms = x[29];
   if (rows <= 0 || B <= 0) return 0;
   int shift = 4;
   while (shift < 7 && 1 << shift != page_size) ++shift;
-  const uintptr_t bases = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache) |
-                          reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work);
-  if (1 << shift != page_size || (bases & 15) != 0 || ((q_row | q_head | k_row | k_head | v_row | v_head | out_row) & 7) != 0 || !(scale > 0.f) ||
-      num_slots <= 0 || max_pages <= 0)
+  if (1 << shift != page_size || ((x[0] | x[1] | x[2] | x[8] | x[9]) & 15) != 0 || ((q_row | q_head | k_row | k_head | v_row | v_head | out_row) & 7) != 0 ||
+      !(scale > 0.f) || num_slots <= 0 || max_pages <= 0)
     return -1;
   sb::TtPlan p;
   if (!sb::tree_attn_plan(B, Hq, Hkv, D, max_nodes, static_cast<long>(max_pages) * page_size, whole, sms, p)) return -1;
-  if (p.bytes > work_bytes) return (int)cudaErrorInvalidValue;
+  if (p.bytes > x[28]) return (int)cudaErrorInvalidValue;
   sb::TtArgs a = {};
-  a.table = table; a.context = context; a.cu = cu; a.parents = parents; a.sinks = sinks;
-  a.out = reinterpret_cast<__nv_bfloat16*>(out);
-  a.plan = reinterpret_cast<int4*>(work);
+  a.table = reinterpret_cast<const int*>(x[3]);
+  a.context = reinterpret_cast<const int*>(x[4]);
+  a.cu = reinterpret_cast<const int*>(x[5]);
+  a.parents = reinterpret_cast<const int*>(x[6]);
+  a.sinks = reinterpret_cast<const float*>(x[7]);
+  a.out = reinterpret_cast<__nv_bfloat16*>(x[8]);
+  a.plan = reinterpret_cast<int4*>(x[9]);
+  a.status = reinterpret_cast<int*>(x[10]);
   a.part_o = reinterpret_cast<float*>(a.plan + 2l * p.ctas);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + 2l * p.ctas * 128 * p.tiles * D);
   a.rows = rows; a.B = B; a.Hkv = Hkv; a.G = Hq / Hkv; a.bq = p.bq; a.page_shift = shift; a.max_pages = max_pages; a.num_slots = num_slots;
   a.max_nodes = max_nodes; a.pairs = p.pairs; a.whole = whole;
   a.out_row = out_row;
   a.c_log2 = scale * 1.4426950408889634f;
-  a.status = status;
   try {
-    const CUtensorMap tq = sb::make_tmap_3d(q, D, Hq, rows, q_head, q_row, 64, a.G, a.bq);
-    const CUtensorMap tk = sb::make_tmap_3d(k_cache, D, Hkv, num_slots, k_head, k_row, 64, 1, page_size);
-    const CUtensorMap tv = sb::make_tmap_3d(v_cache, D, Hkv, num_slots, v_head, v_row, 64, 1, page_size);
+    const CUtensorMap tq = sb::make_tmap_3d(reinterpret_cast<const void*>(x[0]), D, Hq, rows, q_head, q_row, 64, a.G, a.bq);
+    const CUtensorMap tk = sb::make_tmap_3d(reinterpret_cast<const void*>(x[1]), D, Hkv, num_slots, k_head, k_row, 64, 1, page_size);
+    const CUtensorMap tv = sb::make_tmap_3d(reinterpret_cast<const void*>(x[2]), D, Hkv, num_slots, v_head, v_row, 64, 1, page_size);
     auto by_form = [&](auto launch64, auto launch128) { return D == 64 ? launch64(tq, tk, tv, a, p.ctas, s) : launch128(tq, tk, tv, a, p.ctas, s); };
     if (p.tiles == 2) return by_form(sb::launch_tree_attn<64, 2, 1>, sb::launch_tree_attn<128, 2, 1>);
     if (p.copies == 4) return by_form(sb::launch_tree_attn<64, 1, 4>, sb::launch_tree_attn<128, 1, 4>);

@@ -95,10 +95,10 @@ _SIGS = {
     "sb_pg_loss": [P, P, P, P, P, P, P, P, I, F, F, F, I, P],
     "sb_sample": [P, I, L, I, I, P, P, P, P, P, P, P, P, P, P, I, P],
     "sb_tree_attn": [P] * 9 + [I] * 9 + [L] * 7 + [F, I, P],
-    "sb_adjust_logits": [P] * 14 + [L] * 5 + [I] * 6 + [P],
+    "sb_adjust_logits": [P, P],
     "sb_tree_attn_plan": [I, I, I, I, I, L, I, I, P],
-    "sb_tree_attn_tc": [P] * 9 + [I] * 9 + [L] * 7 + [F, I, P, L, I, P, P],
-    "sb_tree_accept": [P, P, P, P, P, P, P, I, I, I, P, I, I, L, I, I, I, L, P, P, I, I, I, I, P],
+    "sb_tree_attn_tc": [P, F, P],
+    "sb_tree_accept": [P, P],
     "sb_kv_write": [P, P, P, P, P, I, I, I, I, P],
     "sb_rope_kv_write": [P, P, P, P, P, P, P, P, I, I, I, I, I, F, P],
     "sb_decode_prepare": [P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, P],

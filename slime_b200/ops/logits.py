@@ -2,11 +2,14 @@
 
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from slime_b200.ops import _checks, _lib, reference, tree as _tree
 
-P = _lib.ptr
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+_CALL = struct.Struct("25q").pack  # arguments of the C entry
 
 
 def _per_request(op: str, name: str, t, requests: int, device):
@@ -30,26 +33,73 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     a tree of drafted tokens (``slime_b200.ops.tree``), and the drafted tokens of the node and those above it count as answered with. The root is the
     last token of the text already. Rows behind the last tree are left as they are. Without it row r is request r.
     Token ids, lengths and mask words are int32. Everything is worked out in fp32 and rounded once."""
-    op = "adjust_logits"
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{op}: logits are [rows, vocabulary] in bf16 or fp32, not {tuple(logits.shape)} in {logits.dtype}")
+    if logits.dim() != 2 or not (logits.dtype is _BF16 or logits.dtype is _F32):
+        raise ValueError(f"adjust_logits: logits are [rows, vocabulary] in bf16 or fp32, not {tuple(logits.shape)} in {logits.dtype}")
     R, V = logits.shape
-    dev = logits.device
+    dev, dtype = logits.device, logits.dtype
+    drafted, parents, cu_nodes = tree if tree is not None else (None, None, None)
+    S = R if cu_nodes is None else cu_nodes.shape[0] - 1
+    penal = repetition is not None or frequency is not None or presence is not None
+    # (as in ``tree.tree_attention``: one expression for what is in order)
+    fine = (out is None or (out.shape == logits.shape and out.dtype is dtype and out.device == dev and (V <= 1 or out.stride(1) == 1)))
+    if fine and penal:
+        fine = (tokens is not None and lengths is not None and tokens.dim() == 2 and tokens.shape[0] == S and tokens.dtype is _I32 and tokens.device == dev
+                and (tokens.shape[1] <= 1 or tokens.stride(1) == 1) and lengths.shape == (S,) and lengths.dtype is _I32 and lengths.device == dev
+                and lengths.is_contiguous())  # fmt: skip
+        if prompt_lens is not None:
+            fine = fine and prompt_lens.shape == (S,) and prompt_lens.dtype is _I32 and prompt_lens.device == dev and prompt_lens.is_contiguous()
+        for t in (repetition, frequency, presence):
+            fine = fine and (t is None or (t.shape == (S,) and t.dtype is _F32 and t.device == dev and t.is_contiguous()))
+    if fine and (bias_ids is not None or bias_values is not None):
+        fine = (bias_ids is not None and bias_values is not None and bias_ids.dim() == 2 and bias_ids.shape[0] == S and bias_values.shape == bias_ids.shape
+                and bias_ids.dtype is _I32 and bias_values.dtype is _F32 and bias_ids.device == dev and bias_values.device == dev
+                and bias_ids.is_contiguous() and bias_values.is_contiguous())  # fmt: skip
+    if fine and allowed is not None:
+        fine = (allowed.shape == (R, -(-V // 32)) and allowed.dtype is _I32 and allowed.device == dev and (allowed.shape[1] <= 1 or allowed.stride(1) == 1))
+    if not fine or tree is not None:
+        _check(logits, tokens, lengths, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, tree, out, S, penal)
+    if out is None:
+        out = logits.new_empty(R, V)
+    if _checks.enabled():
+        if tree is not None:
+            _tree.check_tree_indices("adjust_logits", R, cu_nodes, _tree.MAX_NODES)
+        if penal:
+            _checks.index_range("adjust_logits", "lengths", lengths, upper=tokens.shape[1] + 1)
+    if not logits.is_cuda:
+        return out.copy_(reference.adjust_logits(logits, tokens, lengths, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, tree, out))
+    if R == 0 or V == 0 or S == 0:
+        return out
+    if dev.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return adjust_logits(logits, tokens, lengths, prompt_lens, repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
+                                 bias_values=bias_values, allowed=allowed, tree=tree, out=out)  # fmt: skip
+    if V > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    K = 0 if bias_ids is None else bias_ids.shape[1]
+    text, pitch = (tokens.shape[1], tokens.stride(0)) if penal else (0, 0)
+    rc = _lib.lib().sb_adjust_logits(
+        _CALL(logits.data_ptr(), out.data_ptr(), at(tokens), at(lengths), at(prompt_lens), at(repetition), at(frequency), at(presence), at(bias_ids),
+              at(bias_values), at(allowed), at(drafted), at(parents), at(cu_nodes), logits.stride(0), out.stride(0), pitch, K,
+              0 if allowed is None else allowed.stride(0), R, S, V, text, K, dtype is _F32), _lib.stream())  # fmt: skip
+    _lib.check(rc, "sb_adjust_logits")
+    return out
+
+
+def _check(logits, tokens, lengths, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, tree, out, S: int, penal: bool):
+    """Raises on what ``adjust_logits`` does not take."""
+    op, dev, (R, V) = "adjust_logits", logits.device, logits.shape
     if tree is not None:
         drafted, parents, cu_nodes = tree
         _tree.check_trees(op, R, cu_nodes, _tree.MAX_NODES, drafted=drafted, parents=parents)
-        S = cu_nodes.shape[0] - 1
-    else:
-        drafted = parents = cu_nodes = None
-        S = R
-    L = 0
-    if repetition is not None or frequency is not None or presence is not None:
+        if cu_nodes.device != dev:
+            raise ValueError(f"{op}: logits on {dev}, trees on {cu_nodes.device}")
+    if penal:
         if tokens is None or lengths is None:
             raise ValueError(f"{op}: penalties need the tokens of the requests and their lengths")
         _tree._shape(op, "tokens", tokens, S, None)
         _tree._shape(op, "lengths", lengths, S)
-        L = tokens.shape[1]
-        if tokens.dtype != torch.int32 or tokens.device != dev or (L > 1 and tokens.stride(1) != 1):
+        if tokens.dtype != _I32 or tokens.device != dev or (tokens.shape[1] > 1 and tokens.stride(1) != 1):
             raise ValueError(f"{op}: tokens must be int32 rows on {dev}")
         _tree._ints(op, dev, lengths=lengths)
         if prompt_lens is not None:
@@ -57,38 +107,17 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
             _tree._ints(op, dev, prompt_lens=prompt_lens)
         for name, t in (("repetition", repetition), ("frequency", frequency), ("presence", presence)):
             _per_request(op, name, t, S, dev)
-        if _checks.enabled():
-            _checks.index_range(op, "lengths", lengths, upper=L + 1)
-    K = 0
     if bias_ids is not None or bias_values is not None:
         if bias_ids is None or bias_values is None:
             raise ValueError(f"{op}: biases are ids and values")
         _tree._shape(op, "bias_ids", bias_ids, S, None)
-        K = bias_ids.shape[1]
-        _tree._shape(op, "bias_values", bias_values, S, K)
+        _tree._shape(op, "bias_values", bias_values, S, bias_ids.shape[1])
         _tree._ints(op, dev, bias_ids=bias_ids)
-        if bias_values.dtype != torch.float32 or bias_values.device != dev or not bias_values.is_contiguous():
+        if bias_values.dtype != _F32 or bias_values.device != dev or not bias_values.is_contiguous():
             raise ValueError(f"{op}: bias_values must be contiguous fp32 on {dev}")
     if allowed is not None:
         _tree._shape(op, "allowed", allowed, R, -(-V // 32))
-        if allowed.dtype != torch.int32 or allowed.device != dev or (allowed.shape[1] > 1 and allowed.stride(1) != 1):
+        if allowed.dtype != _I32 or allowed.device != dev or (allowed.shape[1] > 1 and allowed.stride(1) != 1):
             raise ValueError(f"{op}: allowed must be int32 words on {dev}")
-    if out is None:
-        out = torch.empty(R, V, dtype=logits.dtype, device=dev)
-    elif out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (V > 1 and out.stride(1) != 1):
+    if out is not None and (out.shape != logits.shape or out.dtype != logits.dtype or out.device != dev or (V > 1 and out.stride(1) != 1)):
         raise ValueError(f"{op}: out must be like logits, its rows in one piece")
-    if not logits.is_cuda:
-        return out.copy_(reference.adjust_logits(logits, tokens, lengths, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, tree, out))
-    if R == 0 or V == 0 or (tree is not None and S == 0):
-        return out
-    if dev.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(dev):
-            return adjust_logits(logits, tokens, lengths, prompt_lens, repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
-                                 bias_values=bias_values, allowed=allowed, tree=tree, out=out)  # fmt: skip
-    logits = logits if V == 1 or logits.stride(1) == 1 else logits.contiguous()
-    rc = _lib.lib().sb_adjust_logits(
-        P(logits), P(out), P(tokens), P(lengths), P(prompt_lens), P(repetition), P(frequency), P(presence), P(bias_ids), P(bias_values), P(allowed),
-        P(drafted), P(parents), P(cu_nodes), logits.stride(0), out.stride(0), tokens.stride(0) if L else 0, K,
-        allowed.stride(0) if allowed is not None else 0, R, S, V, L, K, int(logits.dtype == torch.float32), _lib.stream())  # fmt: skip
-    _lib.check(rc, "sb_adjust_logits")
-    return out

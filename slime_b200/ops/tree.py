@@ -21,9 +21,9 @@ whatever was drafted. CPU tensors run the definitions in ``reference``.
 
 from __future__ import annotations
 
-import ctypes
 import functools
 import math
+import struct
 
 import torch
 
@@ -34,9 +34,23 @@ P = _lib.ptr
 MAX_NODES = 128  # of a tree
 
 
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+# Arguments of the C entries, as one array: a call costs some 0.1 us for every argument of its own.
+_ATTENTION = struct.Struct("30q").pack
+_ACCEPT = struct.Struct("23q").pack
+_device_facts = {}  # by number: SMs, address of the status word
+
+
+def _facts(device) -> tuple[int, int]:
+    facts = _device_facts.get(device.index)
+    if facts is None:
+        facts = _device_facts[device.index] = _lib.sm_count(device), _lib.status_word(device).data_ptr()
+    return facts
+
+
 def _ints(op: str, device, **tensors):
     for name, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+        if t.dtype != _I32 or t.device != device or not t.is_contiguous():
             raise ValueError(f"{op}: {name} must be a contiguous int32 tensor on {device}, not {t.dtype} on {t.device}")
 
 
@@ -55,14 +69,46 @@ def check_trees(op: str, rows: int, cu_nodes, max_nodes: int, **per_node):
         if t.dim() != 1 or t.shape[0] != rows:
             raise ValueError(f"{op}: {name} has shape {tuple(t.shape)}, not ({rows},)")
     _ints(op, cu_nodes.device, cu_nodes=cu_nodes, **per_node)
-    if _checks.enabled():
-        _checks.index_range(op, "cu_nodes", cu_nodes, upper=rows + 1)
-        _checks.index_range(op, "tree sizes", cu_nodes[1:] - cu_nodes[:-1], upper=max_nodes + 1)
+
+
+def check_tree_indices(op: str, rows: int, cu_nodes, max_nodes: int):
+    """Debug mode: the trees lie within the rows, and none is larger than promised."""
+    _checks.index_range(op, "cu_nodes", cu_nodes, upper=rows + 1)
+    _checks.index_range(op, "tree sizes", cu_nodes[1:] - cu_nodes[:-1], upper=max_nodes + 1)
+
+
+def _check_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, parents, page_size, max_nodes, sinks, out):
+    """Raises on what ``tree_attention`` does not take."""
+    op = "tree_attention"
+    _shape(op, "q", q, None, None, None)
+    T, Hq, D = q.shape
+    _shape(op, "k_cache", k_cache, None, None, D)
+    Hkv = k_cache.shape[1]
+    _shape(op, "v_cache", v_cache, k_cache.shape[0], Hkv, D)
+    check_trees(op, T, cu_nodes, max_nodes, parents=parents)
+    B = cu_nodes.shape[0] - 1
+    _shape(op, "block_table", block_table, B, None)
+    _shape(op, "context_lens", context_lens, B)
+    _ints(op, q.device, cu_nodes=cu_nodes, block_table=block_table, context_lens=context_lens)
+    if Hkv == 0 or Hq % Hkv or page_size <= 0:
+        raise ValueError(f"{op}: {Hq} query heads over {Hkv} key heads, pages of {page_size} tokens")
+    if q.dtype not in (_BF16, _F32) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"{op}: queries and caches are bf16 or fp32 alike, not {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
+    if k_cache.device != q.device or v_cache.device != q.device:
+        raise ValueError(f"{op}: queries on {q.device}, caches on {k_cache.device} and {v_cache.device}")
+    if D > 256:
+        raise ValueError(f"{op}: heads {D} wide (at most 256)")
+    if sinks is not None:
+        _shape(op, "sinks", sinks, Hq)
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or (out.numel() and (out.stride(2), out.stride(1)) != (1, D))):
+        raise ValueError(f"{op}: out must be like q, with heads side by side")
 
 
 @functools.lru_cache(maxsize=4096)
 def _workspace(B: int, Hq: int, Hkv: int, D: int, max_nodes: int, tokens: int, whole: int, sms: int) -> int:
     """Bytes of workspace of the tensor-core kernel; -1 where it does not cover the call."""
+    import ctypes
+
     size = ctypes.c_long()
     rc = _lib.lib().sb_tree_attn_plan(B, Hq, Hkv, D, max_nodes, tokens, whole, sms, ctypes.byref(size))
     return size.value if rc == 0 else -1
@@ -79,77 +125,76 @@ def tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, par
 
     Keys and values of hidden rows have weight zero and have to be finite where they belong to a tree; what stands in a page behind the
     last node may be anything. bf16, and fp32 throughout; heads up to 256 wide."""
-    op = "tree_attention"
+    kv, dev, dtype, B = k_cache.shape, q.device, q.dtype, context_lens.shape[0]
+    # (one expression for calls that are in order, which is most of what a call costs on the host; the check proper says what is wrong with others)
+    if not (q.dim() == 3 and len(kv) == 3 and v_cache.shape == kv and kv[2] == q.shape[2] <= 256 and kv[1] > 0 and q.shape[1] % kv[1] == 0 and page_size > 0
+            and (dtype is _BF16 or dtype is _F32) and k_cache.dtype is dtype and v_cache.dtype is dtype and k_cache.device == dev and v_cache.device == dev
+            and cu_nodes.dtype is _I32 and parents.dtype is _I32 and block_table.dtype is _I32 and context_lens.dtype is _I32 and cu_nodes.device == dev
+            and parents.device == dev and block_table.device == dev and context_lens.device == dev and cu_nodes.is_contiguous() and parents.is_contiguous()
+            and block_table.is_contiguous() and context_lens.is_contiguous() and cu_nodes.shape == (B + 1,) and parents.shape == q.shape[:1]
+            and block_table.dim() == 2 and block_table.shape[0] == B and context_lens.dim() == 1 and 0 < max_nodes <= MAX_NODES
+            and sinks is None and out is None):  # fmt: skip
+        _check_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, parents, page_size, max_nodes, sinks, out)
     T, Hq, D = q.shape
-    Hkv = k_cache.shape[1]
-    _shape(op, "k_cache", k_cache, None, None, D)
-    _shape(op, "v_cache", v_cache, k_cache.shape[0], Hkv, D)
-    B = cu_nodes.shape[0] - 1
-    check_trees(op, T, cu_nodes, max_nodes, parents=parents)
-    _shape(op, "block_table", block_table, B, None)
-    _shape(op, "context_lens", context_lens, B)
-    _ints(op, q.device, cu_nodes=cu_nodes, block_table=block_table, context_lens=context_lens)
-    if Hkv == 0 or Hq % Hkv or page_size <= 0:
-        raise ValueError(f"{op}: {Hq} query heads over {Hkv} key heads, pages of {page_size} tokens")
-    if q.dtype not in (torch.bfloat16, torch.float32) or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
-        raise ValueError(f"{op}: queries and caches are bf16 or fp32 alike, not {q.dtype}, {k_cache.dtype}, {v_cache.dtype}")
-    if k_cache.device != q.device or v_cache.device != q.device:
-        raise ValueError(f"{op}: queries on {q.device}, caches on {k_cache.device} and {v_cache.device}")
-    if sinks is not None:
-        _shape(op, "sinks", sinks, Hq)
-        sinks = sinks.to(q.device, torch.float32).contiguous()
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or out.stride(2) != 1 or out.stride(1) != D:
-        raise ValueError(f"{op}: out must be like q, with heads side by side")
+        out = q.new_empty(T, Hq, D)
+    if sinks is not None:
+        sinks = sinks.to(dev, _F32).contiguous()
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if _checks.enabled() and B:
-        _checks.paged(op, block_table, context_lens + (cu_nodes[1:] - cu_nodes[:-1]), page_size, k_cache.shape[0])
+        check_tree_indices("tree_attention", T, cu_nodes, max_nodes)
+        _checks.paged("tree_attention", block_table, context_lens + (cu_nodes[1:] - cu_nodes[:-1]), page_size, kv[0])
     if not q.is_cuda:
         return reference.tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, parents, page_size, scale, sinks, out)
     if T == 0 or B == 0:
         return out
-    if q.device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(q.device):
+    if dev.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
             return tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, parents, page_size, max_nodes, scale, sinks, out)
-    q, k_cache, v_cache = (x if x.stride(-1) == 1 else x.contiguous() for x in (q, k_cache, v_cache))
+    if q.stride(2) != 1 or k_cache.stride(2) != 1 or v_cache.stride(2) != 1:
+        q, k_cache, v_cache = (x if x.stride(2) == 1 else x.contiguous() for x in (q, k_cache, v_cache))
+    pages = block_table.shape[1]
+    strides = *q.stride()[:2], *k_cache.stride()[:2], *v_cache.stride()[:2], out.stride(0)
     lib = _lib.lib()
-    if q.dtype == torch.bfloat16 and scale > 0:
-        whole, sms = int(ops.BATCH_INVARIANT), _lib.sm_count(q.device)
-        size = _workspace(B, Hq, Hkv, D, max_nodes, block_table.shape[1] * page_size, whole, sms)
+    if dtype is _BF16 and scale > 0:
+        whole = 1 if ops.BATCH_INVARIANT else 0
+        sms, status = _facts(dev)
+        size = _workspace(B, Hq, kv[1], D, max_nodes, pages * page_size, whole, sms)
         if size >= 0:
-            work = torch.empty(size, dtype=torch.uint8, device=q.device)
-            rc = lib.sb_tree_attn_tc(
-                P(q), P(k_cache), P(v_cache), P(block_table), P(context_lens), P(cu_nodes), P(parents), P(sinks), P(out), T, B, Hq, Hkv, D,
-                page_size, block_table.shape[1], k_cache.shape[0], max_nodes, q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1),
-                v_cache.stride(0), v_cache.stride(1), out.stride(0), scale, whole, P(work), size, sms, P(_lib.status_word(q.device)),
-                _lib.stream())  # fmt: skip
+            work = torch.empty(size, dtype=torch.uint8, device=dev)
+            rc = lib.sb_tree_attn_tc(_ATTENTION(
+                q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), cu_nodes.data_ptr(), parents.data_ptr(),
+                0 if sinks is None else sinks.data_ptr(), out.data_ptr(), work.data_ptr(), status, T, B, Hq, kv[1], D, page_size, pages, kv[0], max_nodes,
+                *strides, whole, size, sms), scale, _lib.stream())  # fmt: skip
             if rc != -1:
                 _lib.check(rc, "sb_tree_attn_tc", 2 - whole)
                 return out
     rc = lib.sb_tree_attn(
-        P(q), P(k_cache), P(v_cache), P(block_table), P(context_lens), P(cu_nodes), P(parents), P(sinks), P(out), T, B, Hq, Hkv, D,
-        page_size, block_table.shape[1], k_cache.shape[0], max_nodes, q.stride(0), q.stride(1), k_cache.stride(0), k_cache.stride(1),
-        v_cache.stride(0), v_cache.stride(1), out.stride(0), scale, int(q.dtype == torch.float32), _lib.stream())  # fmt: skip
-    if rc == -1:
-        raise ValueError(f"{op}: heads {D} wide (at most 256)")
+        P(q), P(k_cache), P(v_cache), P(block_table), P(context_lens), P(cu_nodes), P(parents), P(sinks), P(out), T, B, Hq, kv[1], D,
+        page_size, pages, kv[0], max_nodes, *strides, scale, int(dtype is _F32), _lib.stream())  # fmt: skip
     _lib.check(rc, "sb_tree_attn")
     return out
 
 
-def _slabs(op: str, caches):
-    """The caches as (addresses, slabs behind each address, bytes between them) for every geometry of a slot's row: a stacked tensor
-    [layers, slots, heads, width] is one address, a list of tensors [slots, heads, width] one each."""
+def _check_caches(op: str, caches, block_table, context_lens, page_size, B: int, device):
+    """Raises on caches that cannot be moved in; returns them as (slabs behind an address, bytes between them, slots, bytes of a slot's row, bytes from row to
+    row) -> addresses. A stacked tensor [layers, slots, heads, width] is one address, a tensor [slots, heads, width] one of its own."""
+    if block_table is None or context_lens is None or not page_size or page_size <= 0:
+        raise ValueError(f"{op}: caches come with block_table, context_lens and page_size")
+    _shape(op, "block_table", block_table, B, None)
+    _shape(op, "context_lens", context_lens, B)
+    _ints(op, device, block_table=block_table, context_lens=context_lens)
     groups = {}
     for c in caches:
-        layers, step = 1, 0
-        if c.dim() == 4:
-            layers, step = c.shape[0], c.stride(0) * c.element_size()
-        if c.dim() not in (3, 4) or c.stride(-1) != 1 or (c.shape[-2] > 1 and c.stride(-2) != c.shape[-1]):
+        if c.device != device:
+            raise ValueError(f"{op}: caches and trees are on one device")
+        n, strides, shape = c.element_size(), c.stride(), c.shape
+        if len(shape) not in (3, 4) or strides[-1] != 1 or (shape[-2] > 1 and strides[-2] != shape[-1]):
             raise ValueError(f"{op}: a cache is [layers, slots, heads, width], or a list of [slots, heads, width], each slot's row in one piece")
-        width, pitch = c.shape[-1] * c.shape[-2] * c.element_size(), c.stride(-3) * c.element_size()
+        layers, step = (shape[0], strides[0] * n) if len(shape) == 4 else (1, 0)
+        width = shape[-1] * shape[-2] * n
         if width and layers:  # (a cache of latents has no values)
-            groups.setdefault((layers, step, c.shape[-3], width, pitch), []).append(c.data_ptr())
+            groups.setdefault((layers, step, shape[-3], width, strides[-3] * n), []).append(c.data_ptr())
     return groups
 
 
@@ -164,40 +209,40 @@ def accept_tree(sampled, drafted, parents, cu_nodes, max_nodes: int, *, k_caches
     With caches (a stacked tensor [layers, slots, heads, width] or a sequence of [slots, heads, width] each) the keys and values of the nodes on
     the path move, in place, to positions ``context_lens[b] + 0, 1, 2, ...``, so that the cache holds the accepted tokens in order. No page
     that holds nodes of one request may belong to another."""
-    op = "accept_tree"
-    T, B = sampled.shape[0], cu_nodes.shape[0] - 1
-    check_trees(op, T, cu_nodes, max_nodes, sampled=sampled, drafted=drafted, parents=parents)
-    groups = {}
+    op, dev, rows = "accept_tree", cu_nodes.device, sampled.shape
+    if not (0 < max_nodes <= MAX_NODES and len(rows) == 1 and cu_nodes.dim() == 1 and cu_nodes.shape[0] > 0 and drafted.shape == rows and parents.shape == rows
+            and cu_nodes.dtype is _I32 and sampled.dtype is _I32 and drafted.dtype is _I32 and parents.dtype is _I32 and sampled.device == dev
+            and drafted.device == dev and parents.device == dev and sampled.is_contiguous() and drafted.is_contiguous() and parents.is_contiguous()
+            and cu_nodes.is_contiguous()):  # fmt: skip
+        check_trees(op, rows[0], cu_nodes, max_nodes, sampled=sampled, drafted=drafted, parents=parents)
+    T, B, groups, caches = rows[0], cu_nodes.shape[0] - 1, None, ()
     if k_caches is not None or v_caches is not None:
-        if block_table is None or context_lens is None or not page_size or page_size <= 0:
-            raise ValueError(f"{op}: caches come with block_table, context_lens and page_size")
-        _shape(op, "block_table", block_table, B, None)
-        _shape(op, "context_lens", context_lens, B)
-        _ints(op, cu_nodes.device, block_table=block_table, context_lens=context_lens)
         caches = [c for kind in (k_caches, v_caches) if kind is not None for c in ((kind,) if isinstance(kind, torch.Tensor) else kind)]
-        if any(c.device != cu_nodes.device for c in caches):
-            raise ValueError(f"{op}: caches and trees are on one device")
-        groups = _slabs(op, caches)
-        if _checks.enabled() and B:
-            for _, _, slots, _, _ in groups:
-                _checks.paged(op, block_table, context_lens + (cu_nodes[1:] - cu_nodes[:-1]), page_size, slots)
+        groups = _check_caches(op, caches, block_table, context_lens, page_size, B, dev)
+    if _checks.enabled() and B:
+        check_tree_indices(op, T, cu_nodes, max_nodes)
+        for _, _, slots, _, _ in groups or ():
+            _checks.paged(op, block_table, context_lens + (cu_nodes[1:] - cu_nodes[:-1]), page_size, slots)
     if not sampled.is_cuda:
-        return reference.accept_tree(sampled, drafted, parents, cu_nodes, max_nodes, caches if groups else (), block_table, context_lens, page_size)
-    if sampled.device.index != torch._C._cuda_getDevice():
-        with torch.cuda.device(sampled.device):
+        return reference.accept_tree(sampled, drafted, parents, cu_nodes, max_nodes, caches, block_table, context_lens, page_size)
+    if dev.index != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
             return accept_tree(sampled, drafted, parents, cu_nodes, max_nodes, k_caches=k_caches, v_caches=v_caches, block_table=block_table,
                                context_lens=context_lens, page_size=page_size)  # fmt: skip
-    path = torch.empty(B, max_nodes, dtype=torch.int32, device=sampled.device)
-    tokens, count = torch.empty_like(path), torch.empty(B, dtype=torch.int32, device=sampled.device)
-    sms, stream, first = _lib.sm_count(sampled.device), _lib.stream(), True
-    for (layers, step, slots, width, pitch), bases in groups.items() or [((1, 0, 0, 0, 0), [])]:
+    both = sampled.new_empty(2, B, max_nodes)
+    path, tokens = both.unbind()
+    count = sampled.new_empty(B)
+    first = (sampled.data_ptr(), drafted.data_ptr(), parents.data_ptr(), cu_nodes.data_ptr(), path.data_ptr(), tokens.data_ptr(), count.data_ptr())
+    sms, stream, fn = _facts(dev)[0], _lib.stream(), _lib.lib().sb_tree_accept
+    if not groups:
+        _lib.check(fn(_ACCEPT(*first, 0, 0, T, B, max_nodes, 1, 0, 1, sms, 1, 0, 0, 0, 1, 0, 0), stream), "sb_tree_accept")
+        return path, tokens, count
+    where, writes = (block_table.data_ptr(), context_lens.data_ptr(), T, B, max_nodes, page_size, block_table.shape[1]), 1
+    for (layers, step, slots, width, pitch), bases in groups.items():
         unit = math.gcd(16, width, pitch, step, *bases)
-        for i in range(0, max(1, len(bases)), 128):
+        for i in range(0, len(bases), 128):
             part = bases[i : i + 128]
-            rc = _lib.lib().sb_tree_accept(
-                P(sampled), P(drafted), P(parents), P(cu_nodes), P(path), P(tokens), P(count), T, B, max_nodes,
-                (ctypes.c_ulonglong * len(part))(*part), len(part), layers, step, slots, width // unit, unit, pitch, P(block_table),
-                P(context_lens), page_size or 1, 0 if block_table is None else block_table.shape[1], int(first), sms, stream)  # fmt: skip
-            _lib.check(rc, "sb_tree_accept")
-            first = False
+            call = _ACCEPT(*first, *where, writes, sms, layers, step, slots, width // unit, unit, pitch, len(part)) + struct.pack(f"{len(part)}q", *part)
+            _lib.check(fn(call, stream), "sb_tree_accept")
+            writes = 0
     return path, tokens, count
