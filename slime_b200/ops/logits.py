@@ -9,7 +9,7 @@ import torch
 from slime_b200.ops import _checks, _lib, reference, tree as _tree
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
-_CALL = struct.Struct("25q").pack  # arguments of the C entry
+_CALL = struct.Struct("26q").pack  # arguments of the C entry
 
 
 def _per_request(op: str, name: str, t, requests: int, device):
@@ -81,7 +81,7 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     rc = _lib.lib().sb_adjust_logits(
         _CALL(logits.data_ptr(), out.data_ptr(), at(tokens), at(lengths), at(prompt_lens), at(repetition), at(frequency), at(presence), at(bias_ids),
               at(bias_values), at(allowed), at(drafted), at(parents), at(cu_nodes), logits.stride(0), out.stride(0), pitch, K,
-              0 if allowed is None else allowed.stride(0), R, S, V, text, K, dtype is _F32), _lib.stream())  # fmt: skip
+              0 if allowed is None else allowed.stride(0), R, S, V, text, K, dtype is _F32, _tree._facts(dev)[0]), _lib.stream())  # fmt: skip
     _lib.check(rc, "sb_adjust_logits")
     return out
 
