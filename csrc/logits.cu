@@ -5,10 +5,10 @@
 //   x = x - c * frequency - (c > 0) * presence + sum of the biases of t;   x = -inf where the mask's bit of t is 0
 //
 // Nearly all logits of a row are only copied or masked. So calls of some size take two launches: `logits_mask_kernel` copies and masks at the rate of
-// memory, and `logits_used_kernel` works out the few tokens that were used or have a bias. For that a CTA counts a request's text into a table
-// of 16384 tokens of the vocabulary in shared memory, and each token's first taker works it out for all rows of the request: a request needs
-// no table of the vocabulary's size that would have to be kept, cleared and read, only its text. Small calls take one launch,
-// `logits_kernel`, that keeps a chunk of a row in registers while it counts.
+// memory, and `logits_used_kernel` works out the few tokens that were used or have a bias. For that a CTA counts a request's text in a
+// hash table in shared memory, whose places then are the work list for all rows of the request: a request needs no table of the
+// vocabulary's size that would have to be kept, cleared and read, only its text. Small calls take one launch, `logits_kernel`, that
+// keeps a chunk of a row in registers while it counts.
 // Biases of a token are added up in list order by one thread: nothing depends on an order of arrival. Logits that the mask hides are not read.
 // Everything is worked out in fp32 and rounded once. What bounds it: reading and writing the logits, 16 bytes a thread and access; a row that
 // does not start on such a boundary is cut at the boundaries all the same, and its two ends go element by element.
@@ -36,8 +36,9 @@ struct LogitsArgs {
   long in_row, out_row, tokens_row, bias_row, allowed_row;
   int rows, requests, vocab, text, biases;
   int chunks;             // of the vocabulary
-  int parts, slices;      // of the vocabulary; CTAs that share the rows of a tree
+  int slices;             // CTAs that share the rows of a tree
   int penal;
+  int behind_mask;        // the launch in front of this one is logits_mask_kernel
 };
 
 // 16-byte pieces of a row. A row's places are numbered from the 16-byte boundary at or in front of its start, so that place p is token p - off.
@@ -109,8 +110,8 @@ __device__ __forceinline__ float lg_used(float v, bool seen, int times, float re
   return v + bias;
 }
 
-// Adds the text of a request to a table of the tokens [base, base + size): LG_PROMPT, or 1 for every other time.
-enum : int { LG_PROMPT = 1 << 30, LG_BIAS = 1 << 29, LG_DRAFT = 1 << 28, LG_TAKEN = 1 << 27 };
+// What there is of a token: in the prompt, has a bias, was drafted, and how many times it was answered with. lg_text: each token of a request's text.
+enum : int { LG_PROMPT = 1 << 30, LG_BIAS = 1 << 29, LG_DRAFT = 1 << 28 };
 template <typename F>
 __device__ __forceinline__ void lg_text(const LogitsArgs& a, int req, int threads, const F& each) {
   const int* text = a.tokens + req * a.tokens_row;
@@ -235,7 +236,7 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
       for (int k = 0; k < 4; ++k) {
         const int c = cs[k];
         float v = static_cast<float>(e[q + k]);
-        if (c != 0) v = lg_used(v, (c & ~LG_BIAS) != 0, c & (LG_TAKEN - 1), rep, freq, pres, any_bias ? bias[at + q + k] : 0.f);
+        if (c != 0) v = lg_used(v, (c & ~LG_BIAS) != 0, c & (LG_DRAFT - 1), rep, freq, pres, any_bias ? bias[at + q + k] : 0.f);
         if ((shown >> (q + k) & 1) == 0) v = -INFINITY;
         e[q + k] = static_cast<T>(v);
       }
@@ -271,120 +272,210 @@ logits_mask_kernel(const __grid_constant__ LogitsArgs a) {
   }
 }
 
-constexpr int LG_PART = 16384;       // tokens of a table
-constexpr int LG_USED_THREADS = 512;
-
-template <typename T>
-__global__ void __launch_bounds__(LG_USED_THREADS)
+// The tokens of a request that were used, drafted or have a bias, worked out for every `slices`-th row of the request. They are counted in a hash table
+// of HASH places in shared memory (linear probing, at most three quarters full), whose places then are the work list; a longer text
+// is counted in a table of 2 HASH tokens of the vocabulary at a time instead.
+template <typename T, int HASH>
+__global__ void __launch_bounds__(HASH / 16, HASH == 8192 ? 2 : 1)
 logits_used_kernel(const __grid_constant__ LogitsArgs a) {
-  extern __shared__ __align__(16) int count[];
+  constexpr int THREADS = HASH / 16;
+  extern __shared__ __align__(16) int tables[];
+  int* keys = tables;          // [HASH] token, -1: empty
+  int* hashed = tables + HASH;  // [HASH] what there is of it
+  uint16_t* list = reinterpret_cast<uint16_t*>(tables + 2 * HASH);  // occupied places
+  __shared__ int listed;
   __shared__ int tree_p[TREE_MAX], tree_t[TREE_MAX];
   __shared__ __align__(16) uint4 ways[TREE_MAX];
-  pdl_wait();
-  pdl_launch_dependents();
+  // What is counted was there before the launch in front of this one, which has waited for it: only the rows have to be masked first.
+  if (!a.behind_mask) pdl_wait();
   const int tid = threadIdx.x;
-  const int part = blockIdx.x % a.parts, slice = blockIdx.x / a.parts % a.slices, req = blockIdx.x / (a.parts * a.slices);
+  const int slice = blockIdx.x % a.slices, req = blockIdx.x / a.slices;
   int first = req, until = req + 1, n = 0;
   if (a.cu != nullptr) {
     first = a.cu[req];
     until = min(a.cu[req + 1], a.rows);
     n = min(until - first, TREE_MAX);
   }
-  if (first < 0 || first + slice >= until) return;
   const float rep = a.repetition != nullptr ? a.repetition[req] : 1.f;
   const float freq = a.frequency != nullptr ? a.frequency[req] : 0.f;
   const float pres = a.presence != nullptr ? a.presence[req] : 0.f;
   const bool counts = a.penal && (rep != 1.f || freq != 0.f || pres != 0.f);
   const int K = a.biases;
-  if (!counts && K == 0) return;
-  const int base = part * LG_PART, size = min(LG_PART, a.vocab - base);
+  if (first < 0 || first + slice >= until || (!counts && K == 0)) {
+    pdl_wait();  // (every launch of a chain waits for the one in front of it)
+    return;
+  }
   const int* ids = a.bias_ids + req * a.bias_row;
   const float* values = a.bias_values + req * a.bias_row;
-  auto place = [&](int t) { return t >= base && t - base < size ? t - base : -1; };
-  for (int i = tid; i < LG_PART / 4; i += LG_USED_THREADS) reinterpret_cast<int4*>(count)[i] = make_int4(0, 0, 0, 0);
-  for (int i = tid; counts && i < n; i += LG_USED_THREADS) {
+  const int len = counts ? max(min(a.lengths[req], a.text), 0) : 0;
+  const int prompt = counts && a.prompts != nullptr ? a.prompts[req] : 0;
+  if (tid == 0) listed = 0;
+  const bool direct = static_cast<long>(len) + K + n > HASH / 4 * 3;
+  for (int i = tid; counts && i < n; i += THREADS) {
     tree_p[i] = a.parents[first + i];
     tree_t[i] = a.drafted[first + i];
   }
-  __syncthreads();
-  // ---- what there is of each token
-  int again = 0;
-  if (counts) {
-    const int prompt = a.prompts != nullptr ? a.prompts[req] : 0;
-    lg_text(a, req, LG_USED_THREADS, [&](int i, int t) {
-      if (const int at = place(t); at >= 0) {
-        if (i < prompt) atomicOr(&count[at], LG_PROMPT);
-        else atomicAdd(&count[at], 1);
-      }
-    });
-    if (tid < n) {
-      uint32_t set[4];
-      tree_way_up([&](int j) { return tree_p[j]; }, tid, set);
-      ways[tid] = make_uint4(set[0] & ~1u, set[1], set[2], set[3]);  // (the root is the text's last token)
-      if (const int at = place(tree_t[tid]); tid > 0 && at >= 0) atomicOr(&count[at], LG_DRAFT);
+  const int passes = direct ? (a.vocab + 2 * HASH - 1) / (2 * HASH) : 1;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int base = pass * 2 * HASH;
+    const int4 empty = direct ? make_int4(0, 0, 0, 0) : make_int4(-1, -1, -1, -1);
+    for (int i = tid; i < HASH / 4; i += THREADS) {
+      reinterpret_cast<int4*>(keys)[i] = empty;
+      reinterpret_cast<int4*>(hashed)[i] = make_int4(0, 0, 0, 0);
     }
-  }
-  for (int i = tid; i < K; i += LG_USED_THREADS)
-    if (const int at = place(ids[i]); at >= 0) again |= (atomicOr(&count[at], LG_BIAS) & LG_BIAS) != 0;  // listed twice
-  again = __syncthreads_or(again);
-  // ---- the first to take a token works it out for this CTA's rows. entry: of the list of biases, or -1
-  auto take = [&](int t, int entry) {
-    const int at = place(t);
-    if (at < 0) return;
-    if (count[at] & LG_TAKEN) return;
-    const int c = atomicOr(&count[at], LG_TAKEN);
-    if (c & LG_TAKEN) return;
-    float bias = 0.f;
-    if (c & LG_BIAS) {
-      if (entry >= 0 && !again) {
-        bias = values[entry];
-      } else {
-        for (int j = 0; j < K; ++j)
-          if (ids[j] == t) bias += values[j];
+    __syncthreads();
+    // ---- what there is of each token
+    auto place = [&](int t) -> int* {
+      if (static_cast<unsigned>(t) >= static_cast<unsigned>(a.vocab)) return nullptr;
+      if (direct) return t >= base && t - base < 2 * HASH ? tables + (t - base) : nullptr;
+      unsigned at = (static_cast<unsigned>(t) * 2654435761u) >> 16;  // Knuth's multiplicative hashing
+      while (true) {
+        at &= HASH - 1;
+        const int was = atomicCAS(&keys[at], -1, t);
+        if (was == -1 || was == t) return &hashed[at];
+        ++at;
       }
-    }
-    uint32_t nodes[4] = {0, 0, 0, 0};  // that stand for this token
-    if (c & LG_DRAFT)
-      for (int j = 1; j < n; ++j)
-        if (tree_t[j] == t) {
-#pragma unroll
-          for (int w = 0; w < 4; ++w)
-            if (j >> 5 == w) nodes[w] |= 1u << (j & 31);
+    };
+    if (counts) {
+      lg_text(a, req, THREADS, [&](int i, int t) {
+        if (int* at = place(t); at != nullptr) {
+          if (i < prompt) atomicOr(at, LG_PROMPT);
+          else atomicAdd(at, 1);
         }
-    const int times0 = c & (LG_TAKEN - 1);
-    constexpr int FLY = 4;  // rows whose reads are under way together
-    for (int r0 = first + slice; r0 < until; r0 += FLY * a.slices) {
+      });
+      if (tid < n) {
+        if (pass == 0) {
+          uint32_t set[4];
+          tree_way_up([&](int j) { return tree_p[j]; }, tid, set);
+          ways[tid] = make_uint4(set[0] & ~1u, set[1], set[2], set[3]);  // (the root is the text's last token)
+        }
+        if (tid > 0)
+          if (int* at = place(tree_t[tid]); at != nullptr) atomicOr(at, LG_DRAFT);
+      }
+    }
+    // biases: the first of a token's entries to come works the token out. again: a token is listed twice. mine: entries, one bit each
+    const bool marks = K <= 32 * THREADS;
+    uint32_t mine = 0;
+    int again = 0;
+    for (int i = tid, x = 0; i < K; i += THREADS, ++x)
+      if (int* at = place(ids[i]); at != nullptr) {
+        const bool came = (atomicOr(at, LG_BIAS) & LG_BIAS) == 0;
+        if (came && marks) mine |= 1u << x;
+        again |= !came;
+      }
+    again = __syncthreads_or(again);
+    if (pass == 0) {
+      if (a.behind_mask) pdl_wait();
+      pdl_launch_dependents();
+    }
+    // ---- each token's logits
+    constexpr int FLY = 4;  // logits whose reads are under way together
+    const int step = a.slices, rows = (until - first - slice + step - 1) / step;  // this CTA's rows: first + slice + x step
+    // c 0: nothing to do
+    auto work = [&](const int (&t)[FLY], const int (&c)[FLY], const int (&r)[FLY], float bias) {
       T v[FLY];
       uint32_t word[FLY];
 #pragma unroll
       for (int x = 0; x < FLY; ++x) {
-        const int r = r0 + x * a.slices;
-        word[x] = 0xffffffffu;
-        if (r < until) {
-          v[x] = reinterpret_cast<const T*>(a.in)[r * a.in_row + t];
-          if (a.allowed != nullptr) word[x] = static_cast<uint32_t>(a.allowed[r * a.allowed_row + (t >> 5)]);
-        }
+        word[x] = c[x] != 0 ? 0xffffffffu : 0u;
+        if (c[x] == 0) continue;
+        v[x] = reinterpret_cast<const T*>(a.in)[r[x] * a.in_row + t[x]];
+        if (a.allowed != nullptr) word[x] = static_cast<uint32_t>(a.allowed[r[x] * a.allowed_row + (t[x] >> 5)]);
       }
 #pragma unroll
       for (int x = 0; x < FLY; ++x) {
-        const int r = r0 + x * a.slices;
-        if (r >= until) break;
-        int times = times0;
-        if ((c & LG_DRAFT) && r - first < n) {
-          const uint4 w = ways[r - first];
-          times += __popc(w.x & nodes[0]) + __popc(w.y & nodes[1]) + __popc(w.z & nodes[2]) + __popc(w.w & nodes[3]);
+        if ((word[x] >> (t[x] & 31) & 1) == 0) continue;  // (hidden: -infinity already)
+        int times = c[x] & (LG_DRAFT - 1);
+        if ((c[x] & LG_DRAFT) && r[x] - first < n) {
+          const uint32_t* way = reinterpret_cast<const uint32_t*>(&ways[r[x] - first]);
+          for (int j = 1; j < n; ++j) times += tree_t[j] == t[x] && (way[j >> 5] >> (j & 31) & 1);
         }
-        if ((word[x] >> (t & 31) & 1) == 0) continue;  // (-infinity already)
-        const float y = lg_used(static_cast<float>(v[x]), times > 0 || (c & LG_PROMPT), times, rep, freq, pres, bias);
-        reinterpret_cast<T*>(a.out)[r * a.out_row + t] = static_cast<T>(y);
+        const float y = lg_used(static_cast<float>(v[x]), times > 0 || (c[x] & LG_PROMPT), times, rep, freq, pres, bias);
+        reinterpret_cast<T*>(a.out)[r[x] * a.out_row + t[x]] = static_cast<T>(y);
+      }
+    };
+    if (!direct) {
+      // the occupied places side by side; (place, row) pairs are dealt out evenly
+      for (int p0 = 0; p0 < HASH; p0 += THREADS) {
+        const int c = hashed[p0 + tid];
+        const bool some = c != 0 && (c & LG_BIAS) == 0;
+        const uint32_t all = __ballot_sync(0xffffffffu, some);
+        int at = 0;
+        if ((tid & 31) == 0 && all != 0) at = atomicAdd(&listed, __popc(all));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << (tid & 31)) - 1));
+        if (some) list[at] = static_cast<uint16_t>(p0 + tid);
+      }
+      __syncthreads();
+      const int m = listed;
+      for (int p0 = tid; p0 < m * rows; p0 += FLY * THREADS) {
+        int t[FLY], c[FLY], r[FLY];
+#pragma unroll
+        for (int x = 0; x < FLY; ++x) {
+          const int p = p0 + x * THREADS;
+          const bool some = p < m * rows;
+          const int row = some ? p / m : 0, at = some ? list[p - row * m] : 0;
+          t[x] = some ? keys[at] : 0;
+          c[x] = some ? hashed[at] : 0;
+          r[x] = first + slice + row * step;
+        }
+        work(t, c, r, 0.f);
+      }
+    } else {
+      for (int p0 = tid; p0 < 2 * HASH; p0 += FLY * THREADS) {
+        int t[FLY], c[FLY];
+#pragma unroll
+        for (int x = 0; x < FLY; ++x) {
+          const int at = p0 + x * THREADS;
+          t[x] = base + at;
+          c[x] = tables[at];
+          if (c[x] & LG_BIAS) c[x] = 0;
+        }
+        if ((c[0] | c[1] | c[2] | c[3]) != 0)
+          for (int r0 = first + slice; r0 < until; r0 += step) {
+            const int r[FLY] = {r0, r0, r0, r0};
+            work(t, c, r, 0.f);
+          }
       }
     }
-  };
-  for (int i = tid; i < K; i += LG_USED_THREADS) take(ids[i], i);
-  if (counts) {
-    if (tid > 0 && tid < n) take(tree_t[tid], -1);
-    lg_text(a, req, LG_USED_THREADS, [&](int, int t) { take(t, -1); });
+    for (int i = tid, x = 0; i < K; i += THREADS, ++x) {
+      const int id = ids[i];
+      if (marks && (mine >> x & 1) == 0) continue;
+      const int* at = place(id);
+      if (at == nullptr) continue;
+      bool leads = true;
+      for (int j = 0; !marks && leads && j < i; ++j) leads = ids[j] != id;
+      if (!leads) continue;
+      float bias = values[i];
+      if (again) {
+        bias = 0.f;
+        for (int j = 0; j < K; ++j)
+          if (ids[j] == id) bias += values[j];
+      }
+      const int what = *at, t[FLY] = {id, id, id, id};
+      for (int r0 = first + slice; r0 < until; r0 += FLY * step) {
+        int c[FLY], r[FLY];
+#pragma unroll
+        for (int y = 0; y < FLY; ++y) {
+          r[y] = r0 + y * step;
+          c[y] = r[y] < until ? what : 0;
+        }
+        work(t, c, r, bias);
+      }
+    }
+    if (pass + 1 < passes) __syncthreads();
   }
+}
+
+template <typename T, int HASH>
+static int launch_used(LogitsArgs a, int sms, cudaStream_t s) {
+  // CTAs that share the rows of a tree: each counts the text for itself
+  a.slices = a.cu == nullptr ? 1 : static_cast<int>(a.requests >= 2l * sms ? 1 : 2l * sms / a.requests);
+  if (a.slices > 8) a.slices = 8;
+  if (static_cast<long>(a.requests) * a.slices > 0x7fffffffl) return (int)cudaErrorInvalidValue;
+  auto kern = logits_used_kernel<T, HASH>;
+  constexpr int bytes = 2 * HASH * 4 + HASH / 4 * 3 * 2;
+  if (cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), bytes); e != cudaSuccess) return (int)e;
+  return (int)launch_pdl(kern, dim3(a.requests * a.slices), dim3(HASH / 16), bytes, s, a);
 }
 
 template <typename T>
@@ -401,16 +492,11 @@ static int launch_logits(LogitsArgs a, int sms, cudaStream_t s) {
     const long ctas = static_cast<long>(a.chunks) * a.rows;
     if (ctas > 0x7fffffffl) return (int)cudaErrorInvalidValue;
     if (cudaError_t e = launch_pdl(logits_mask_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(LG_THREADS), 0, s, a); e != cudaSuccess) return (int)e;
+    a.behind_mask = 1;
   }
   if (!used) return 0;
-  a.parts = (a.vocab + LG_PART - 1) / LG_PART;
-  // CTAs that share the rows of a tree: each counts the text for itself
-  const long ctas = static_cast<long>(a.parts) * a.requests;
-  a.slices = a.cu == nullptr ? 1 : static_cast<int>(ctas >= 6L * sms ? 1 : (6L * sms + ctas - 1) / ctas);
-  if (a.slices > 8) a.slices = 8;
-  if (ctas * a.slices > 0x7fffffffl) return (int)cudaErrorInvalidValue;
-  if (cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(logits_used_kernel<T>), LG_PART * 4); e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(logits_used_kernel<T>, dim3(static_cast<unsigned>(ctas * a.slices)), dim3(LG_USED_THREADS), LG_PART * 4, s, a);
+  // 64 KB of table leave room for three CTAs on an SM, 128 KB take a text of 12,000 tokens
+  return static_cast<long>(a.text) + a.biases + TREE_MAX <= 6144 ? launch_used<T, 8192>(a, sms, s) : launch_used<T, 16384>(a, sms, s);
 }
 
 }  // namespace sb
