@@ -4,11 +4,11 @@
 //   x = seen ? (x > 0 ? x / repetition : x * repetition) : x
 //   x = x - c * frequency - (c > 0) * presence + sum of the biases of t;   x = -inf where the mask's bit of t is 0
 //
-// Nearly all logits of a row are only copied or masked. So calls of some size take two launches: `logits_mask_kernel` copies and masks at the rate of
-// memory, and `logits_used_kernel` works out the few tokens that were used or have a bias. For that a CTA counts a request's text in a
-// hash table in shared memory, whose places then are the work list for all rows of the request: a request needs no table of the
-// vocabulary's size that would have to be kept, cleared and read, only its text. Small calls take one launch, `logits_kernel`, that
-// keeps a chunk of a row in registers while it counts.
+// Nearly all logits of a row are only copied or masked. So a call of some size takes two launches: `logits_count_kernel` counts each request's text in a
+// hash table in shared memory and lists the few tokens that were used or have a bias, `logits_row_kernel` copies and masks the rows at the rate of
+// memory and puts in the listed ones while their lines are near. A request needs no table of the vocabulary's size that would have to be
+// kept, cleared and read, only its text. (Putting them in behind the whole copy cost 55 us of 195 at 763 rows of 151936: single
+// words to lines that had left the L2.) A small call takes one launch, `logits_kernel`, that keeps a chunk of a row in registers while it counts.
 // Biases of a token are added up in list order by one thread: nothing depends on an order of arrival. Logits that the mask hides are not read.
 // Everything is worked out in fp32 and rounded once. What bounds it: reading and writing the logits, 16 bytes a thread and access; a row that
 // does not start on such a boundary is cut at the boundaries all the same, and its two ends go element by element.
@@ -17,6 +17,7 @@
 namespace sb {
 
 constexpr int LG_THREADS = 256;
+constexpr int LG_BUCKETS = 1024;
 
 struct LogitsArgs {
   const void* in;
@@ -36,9 +37,17 @@ struct LogitsArgs {
   long in_row, out_row, tokens_row, bias_row, allowed_row;
   int rows, requests, vocab, text, biases;
   int chunks;             // of the vocabulary
-  int slices;             // CTAs that share the rows of a tree
   int penal;
-  int behind_mask;        // the launch in front of this one is logits_mask_kernel
+  // what logits_count_kernel leaves for logits_row_kernel: of each row of a tree the nodes on its way and its request; of each request the tokens
+  // to work out, what there is of them and their biases, by bucket of 2^bucket_shift tokens
+  int listed, bucket_shift;
+  long list_room;
+  uint4* row_way;
+  int* row_request;
+  int* list_start;        // [S, buckets + 1]
+  int* list_token;        // [S, list_room]
+  int* list_what;
+  float* list_bias;
 };
 
 // 16-byte pieces of a row. A row's places are numbered from the 16-byte boundary at or in front of its start, so that place p is token p - off.
@@ -245,77 +254,58 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
   }
 }
 
-// ---------------------------------------------------------------- two launches: copy and mask; then the tokens that were used or have a bias
-template <typename T>
-__global__ void __launch_bounds__(LG_THREADS)
-logits_mask_kernel(const __grid_constant__ LogitsArgs a) {
-  constexpr int NV = 4, E = 16 / sizeof(T);
-  pdl_wait();
-  pdl_launch_dependents();
-  const int r = blockIdx.x / a.chunks, chunk = blockIdx.x - r * a.chunks;
-  if (a.cu != nullptr && (r < a.cu[0] || r >= a.cu[a.requests])) return;  // not a row of a tree: left as it is
-  Pieces<T, NV> x;
-  x.load(a, r, chunk * (NV * E * LG_THREADS));
-  const bool in_place = a.in == a.out && a.in_row == a.out_row;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int t0 = x.token(i);
-    const uint32_t shown = x.shown(i);
-    if (t0 + E <= 0 || t0 >= a.vocab || (in_place && shown == (1u << E) - 1)) continue;
-    if (shown != (1u << E) - 1) {
-      T* e = reinterpret_cast<T*>(&x.x[i]);
-#pragma unroll
-      for (int k = 0; k < E; ++k)
-        if ((shown >> k & 1) == 0) e[k] = static_cast<T>(-INFINITY);
-    }
-    x.store(a, i);
-  }
-}
-
-// The tokens of a request that were used, drafted or have a bias, worked out for every `slices`-th row of the request. They are counted in a hash table
-// of HASH places in shared memory (linear probing, at most three quarters full), whose places then are the work list; a longer text
-// is counted in a table of 2 HASH tokens of the vocabulary at a time instead.
-template <typename T, int HASH>
-__global__ void __launch_bounds__(HASH / 16, HASH == 8192 ? 2 : 1)
-logits_used_kernel(const __grid_constant__ LogitsArgs a) {
+// ---------------------------------------------------------------- two launches: count; then copy, mask and put in what was counted
+// Lists the tokens of a request that were used, drafted or have a bias, by bucket of the vocabulary. They are counted in a hash table of HASH places
+// in shared memory (linear probing, at most three quarters full); a longer text is counted in a table of 2 HASH tokens of the vocabulary at a time.
+template <int HASH>
+__global__ void __launch_bounds__(HASH / 16, HASH == 8192 ? 3 : 1)
+logits_count_kernel(const __grid_constant__ LogitsArgs a) {
   constexpr int THREADS = HASH / 16;
   extern __shared__ __align__(16) int tables[];
   int* keys = tables;          // [HASH] token, -1: empty
   int* hashed = tables + HASH;  // [HASH] what there is of it
-  uint16_t* list = reinterpret_cast<uint16_t*>(tables + 2 * HASH);  // occupied places
-  __shared__ int listed;
   __shared__ int tree_p[TREE_MAX], tree_t[TREE_MAX];
-  __shared__ __align__(16) uint4 ways[TREE_MAX];
-  // What is counted was there before the launch in front of this one, which has waited for it: only the rows have to be masked first.
-  if (!a.behind_mask) pdl_wait();
-  const int tid = threadIdx.x;
-  const int slice = blockIdx.x % a.slices, req = blockIdx.x / a.slices;
-  int first = req, until = req + 1, n = 0;
+  __shared__ int start[LG_BUCKETS + 1];  // places in the list: how many of a bucket, then where the next one goes
+  __shared__ int sums[32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, req = blockIdx.x;
+  int first = 0, until = 0, n = 0;
   if (a.cu != nullptr) {
     first = a.cu[req];
     until = min(a.cu[req + 1], a.rows);
-    n = min(until - first, TREE_MAX);
+    n = first < 0 ? 0 : max(min(until - first, TREE_MAX), 0);
   }
   const float rep = a.repetition != nullptr ? a.repetition[req] : 1.f;
   const float freq = a.frequency != nullptr ? a.frequency[req] : 0.f;
   const float pres = a.presence != nullptr ? a.presence[req] : 0.f;
   const bool counts = a.penal && (rep != 1.f || freq != 0.f || pres != 0.f);
   const int K = a.biases;
-  if (first < 0 || first + slice >= until || (!counts && K == 0)) {
-    pdl_wait();  // (every launch of a chain waits for the one in front of it)
-    return;
-  }
   const int* ids = a.bias_ids + req * a.bias_row;
   const float* values = a.bias_values + req * a.bias_row;
   const int len = counts ? max(min(a.lengths[req], a.text), 0) : 0;
   const int prompt = counts && a.prompts != nullptr ? a.prompts[req] : 0;
-  if (tid == 0) listed = 0;
   const bool direct = static_cast<long>(len) + K + n > HASH / 4 * 3;
-  for (int i = tid; counts && i < n; i += THREADS) {
+  for (int i = tid; i < n; i += THREADS) {
     tree_p[i] = a.parents[first + i];
     tree_t[i] = a.drafted[first + i];
   }
+  __syncthreads();
+  if (first >= 0)
+    for (int r = first + tid; r < until; r += THREADS) {  // rows of the tree: whose they are, and the nodes on the way to them (the root is the text's last token)
+      uint32_t set[4] = {0, 0, 0, 0};
+      if (r - first < n) tree_way_up([&](int j) { return tree_p[j]; }, r - first, set);
+      a.row_way[r] = make_uint4(set[0] & ~1u, set[1], set[2], set[3]);
+      a.row_request[r] = req;
+    }
+  const int buckets = ((a.vocab - 1) >> a.bucket_shift) + 1;
+  int* list_start = a.list_start + static_cast<long>(req) * (buckets + 1);
+  int* list_token = a.list_token + static_cast<long>(req) * a.list_room;
+  int* list_what = a.list_what + static_cast<long>(req) * a.list_room;
+  float* list_bias = a.list_bias + static_cast<long>(req) * a.list_room;
   const int passes = direct ? (a.vocab + 2 * HASH - 1) / (2 * HASH) : 1;
+  for (int i = tid; i < buckets; i += THREADS) start[i] = 0;
+  int listed = 0;  // by the passes before
   for (int pass = 0; pass < passes; ++pass) {
     const int base = pass * 2 * HASH;
     const int4 empty = direct ? make_int4(0, 0, 0, 0) : make_int4(-1, -1, -1, -1);
@@ -343,17 +333,10 @@ logits_used_kernel(const __grid_constant__ LogitsArgs a) {
           else atomicAdd(at, 1);
         }
       });
-      if (tid < n) {
-        if (pass == 0) {
-          uint32_t set[4];
-          tree_way_up([&](int j) { return tree_p[j]; }, tid, set);
-          ways[tid] = make_uint4(set[0] & ~1u, set[1], set[2], set[3]);  // (the root is the text's last token)
-        }
-        if (tid > 0)
-          if (int* at = place(tree_t[tid]); at != nullptr) atomicOr(at, LG_DRAFT);
-      }
+      if (tid > 0 && tid < n)
+        if (int* at = place(tree_t[tid]); at != nullptr) atomicOr(at, LG_DRAFT);
     }
-    // biases: the first of a token's entries to come works the token out. again: a token is listed twice. mine: entries, one bit each
+    // biases: the first of a token's entries to come lists the token. again: a token is listed twice. mine: entries, one bit each
     const bool marks = K <= 32 * THREADS;
     uint32_t mine = 0;
     int again = 0;
@@ -364,79 +347,42 @@ logits_used_kernel(const __grid_constant__ LogitsArgs a) {
         again |= !came;
       }
     again = __syncthreads_or(again);
-    if (pass == 0) {
-      if (a.behind_mask) pdl_wait();
-      pdl_launch_dependents();
-    }
-    // ---- each token's logits
-    constexpr int FLY = 4;  // logits whose reads are under way together
-    const int step = a.slices, rows = (until - first - slice + step - 1) / step;  // this CTA's rows: first + slice + x step
-    // c 0: nothing to do
-    auto work = [&](const int (&t)[FLY], const int (&c)[FLY], const int (&r)[FLY], float bias) {
-      T v[FLY];
-      uint32_t word[FLY];
+    // ---- by bucket: how many there are, where each bucket begins, then the tokens (in any order within a bucket)
+    const int places = direct ? 2 * HASH : HASH;
+    auto token_at = [&](int at) { return direct ? base + at : keys[at]; };
+    auto what_at = [&](int at) { return direct ? tables[at] : hashed[at]; };
+    for (int at = tid; at < places; at += THREADS)
+      if (what_at(at) != 0) atomicAdd(&start[token_at(at) >> a.bucket_shift], 1);
+    __syncthreads();
+    const int b0 = direct ? base >> a.bucket_shift : 0, b1 = direct ? min(buckets, (base + 2 * HASH) >> a.bucket_shift) : buckets;  // of this pass
+    for (int from = b0; from < b1; from += THREADS) {
+      const int b = from + tid, mine_b = b < b1 ? start[b] : 0;
+      int incl = mine_b;
 #pragma unroll
-      for (int x = 0; x < FLY; ++x) {
-        word[x] = c[x] != 0 ? 0xffffffffu : 0u;
-        if (c[x] == 0) continue;
-        v[x] = reinterpret_cast<const T*>(a.in)[r[x] * a.in_row + t[x]];
-        if (a.allowed != nullptr) word[x] = static_cast<uint32_t>(a.allowed[r[x] * a.allowed_row + (t[x] >> 5)]);
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
       }
-#pragma unroll
-      for (int x = 0; x < FLY; ++x) {
-        if ((word[x] >> (t[x] & 31) & 1) == 0) continue;  // (hidden: -infinity already)
-        int times = c[x] & (LG_DRAFT - 1);
-        if ((c[x] & LG_DRAFT) && r[x] - first < n) {
-          const uint32_t* way = reinterpret_cast<const uint32_t*>(&ways[r[x] - first]);
-          for (int j = 1; j < n; ++j) times += tree_t[j] == t[x] && (way[j >> 5] >> (j & 31) & 1);
-        }
-        const float y = lg_used(static_cast<float>(v[x]), times > 0 || (c[x] & LG_PROMPT), times, rep, freq, pres, bias);
-        reinterpret_cast<T*>(a.out)[r[x] * a.out_row + t[x]] = static_cast<T>(y);
-      }
-    };
-    if (!direct) {
-      // the occupied places side by side; (place, row) pairs are dealt out evenly
-      for (int p0 = 0; p0 < HASH; p0 += THREADS) {
-        const int c = hashed[p0 + tid];
-        const bool some = c != 0 && (c & LG_BIAS) == 0;
-        const uint32_t all = __ballot_sync(0xffffffffu, some);
-        int at = 0;
-        if ((tid & 31) == 0 && all != 0) at = atomicAdd(&listed, __popc(all));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(all & ((1u << (tid & 31)) - 1));
-        if (some) list[at] = static_cast<uint16_t>(p0 + tid);
-      }
+      if (lane == 31) sums[warp] = incl;
       __syncthreads();
-      const int m = listed;
-      for (int p0 = tid; p0 < m * rows; p0 += FLY * THREADS) {
-        int t[FLY], c[FLY], r[FLY];
-#pragma unroll
-        for (int x = 0; x < FLY; ++x) {
-          const int p = p0 + x * THREADS;
-          const bool some = p < m * rows;
-          const int row = some ? p / m : 0, at = some ? list[p - row * m] : 0;
-          t[x] = some ? keys[at] : 0;
-          c[x] = some ? hashed[at] : 0;
-          r[x] = first + slice + row * step;
-        }
-        work(t, c, r, 0.f);
+      int before = listed, total = 0;
+      for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) before += sums[w];
+        total += sums[w];
       }
-    } else {
-      for (int p0 = tid; p0 < 2 * HASH; p0 += FLY * THREADS) {
-        int t[FLY], c[FLY];
-#pragma unroll
-        for (int x = 0; x < FLY; ++x) {
-          const int at = p0 + x * THREADS;
-          t[x] = base + at;
-          c[x] = tables[at];
-          if (c[x] & LG_BIAS) c[x] = 0;
-        }
-        if ((c[0] | c[1] | c[2] | c[3]) != 0)
-          for (int r0 = first + slice; r0 < until; r0 += step) {
-            const int r[FLY] = {r0, r0, r0, r0};
-            work(t, c, r, 0.f);
-          }
-      }
+      if (b < b1) start[b] = list_start[b] = before + incl - mine_b;
+      listed += total;
+      __syncthreads();
     }
+    if (pass + 1 == passes && tid == 0) list_start[buckets] = listed;
+    auto put = [&](int t, int what, float bias) {
+      const int at = atomicAdd(&start[t >> a.bucket_shift], 1);
+      list_token[at] = t;
+      list_what[at] = what;
+      list_bias[at] = bias;
+    };
+    for (int at = tid; at < places; at += THREADS)
+      if (const int what = what_at(at); what != 0 && (what & LG_BIAS) == 0) put(token_at(at), what, 0.f);
     for (int i = tid, x = 0; i < K; i += THREADS, ++x) {
       const int id = ids[i];
       if (marks && (mine >> x & 1) == 0) continue;
@@ -451,59 +397,137 @@ logits_used_kernel(const __grid_constant__ LogitsArgs a) {
         for (int j = 0; j < K; ++j)
           if (ids[j] == id) bias += values[j];
       }
-      const int what = *at, t[FLY] = {id, id, id, id};
-      for (int r0 = first + slice; r0 < until; r0 += FLY * step) {
-        int c[FLY], r[FLY];
-#pragma unroll
-        for (int y = 0; y < FLY; ++y) {
-          r[y] = r0 + y * step;
-          c[y] = r[y] < until ? what : 0;
-        }
-        work(t, c, r, bias);
-      }
+      put(id, *at, bias);
     }
     if (pass + 1 < passes) __syncthreads();
   }
 }
 
-template <typename T, int HASH>
-static int launch_used(LogitsArgs a, int sms, cudaStream_t s) {
-  // CTAs that share the rows of a tree: each counts the text for itself
-  a.slices = a.cu == nullptr ? 1 : static_cast<int>(a.requests >= 2l * sms ? 1 : 2l * sms / a.requests);
-  if (a.slices > 8) a.slices = 8;
-  if (static_cast<long>(a.requests) * a.slices > 0x7fffffffl) return (int)cudaErrorInvalidValue;
-  auto kern = logits_used_kernel<T, HASH>;
-  constexpr int bytes = 2 * HASH * 4 + HASH / 4 * 3 * 2;
-  if (cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), bytes); e != cudaSuccess) return (int)e;
-  return (int)launch_pdl(kern, dim3(a.requests * a.slices), dim3(HASH / 16), bytes, s, a);
+// Copies and masks a chunk of a row, then puts in the logits of the listed tokens (their lines have just been here).
+template <typename T>
+__global__ void __launch_bounds__(LG_THREADS)
+logits_row_kernel(const __grid_constant__ LogitsArgs a) {
+  constexpr int NV = 4, E = 16 / sizeof(T), CHUNK = NV * E * LG_THREADS;
+  // The rows were there before the launch in front of this one, which has waited for them: only the lists have to be waited for.
+  if (!a.listed) pdl_wait();
+  const int tid = threadIdx.x;
+  const int r = blockIdx.x / a.chunks, chunk = blockIdx.x - r * a.chunks;
+  if (a.cu != nullptr && (r < a.cu[0] || r >= a.cu[a.requests])) {  // not a row of a tree: left as it is
+    pdl_wait();
+    return;
+  }
+  Pieces<T, NV> x;
+  x.load(a, r, chunk * CHUNK);
+  if (a.listed) pdl_wait();
+  pdl_launch_dependents();
+  const int lo = max(x.base, 0), hi = min(x.base + CHUNK, a.vocab);  // the chunk's tokens
+  int req = r, from = 0, until = 0;
+  long room = 0;
+  if (a.listed && lo < hi) {
+    if (a.cu != nullptr) req = a.row_request[r];
+    const int buckets = ((a.vocab - 1) >> a.bucket_shift) + 1;
+    const int* list_start = a.list_start + static_cast<long>(req) * (buckets + 1);
+    from = list_start[lo >> a.bucket_shift];
+    until = list_start[((hi - 1) >> a.bucket_shift) + 1];
+    room = static_cast<long>(req) * a.list_room;
+  }
+  const bool in_place = a.in == a.out && a.in_row == a.out_row;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int t0 = x.token(i);
+    const uint32_t shown = x.shown(i);
+    if (t0 + E <= 0 || t0 >= a.vocab || (in_place && shown == (1u << E) - 1)) continue;
+    if (shown != (1u << E) - 1) {
+      T* e = reinterpret_cast<T*>(&x.x[i]);
+#pragma unroll
+      for (int k = 0; k < E; ++k)
+        if ((shown >> k & 1) == 0) e[k] = static_cast<T>(-INFINITY);
+    }
+    x.store(a, i);
+  }
+  if (from >= until) return;
+  __syncthreads();
+  const float rep = a.repetition != nullptr ? a.repetition[req] : 1.f;
+  const float freq = a.frequency != nullptr ? a.frequency[req] : 0.f;
+  const float pres = a.presence != nullptr ? a.presence[req] : 0.f;
+  for (int i = from + tid; i < until; i += LG_THREADS) {
+    const int t = a.list_token[room + i], what = a.list_what[room + i];
+    if (t < lo || t >= hi) continue;
+    if (a.allowed != nullptr && (a.allowed[r * a.allowed_row + (t >> 5)] >> (t & 31) & 1) == 0) continue;  // (hidden: -infinity already)
+    int times = what & (LG_DRAFT - 1);
+    if (what & LG_DRAFT) {  // drafted nodes of this token on the way to this row
+      const uint4 way = a.row_way[r];
+      const int first = a.cu[req], n = min(min(a.cu[req + 1], a.rows) - first, TREE_MAX);
+      for (int j = 1; j < n; ++j) {
+        const uint32_t word = j < 32 ? way.x : j < 64 ? way.y : j < 96 ? way.z : way.w;
+        if (word >> (j & 31) & 1) times += a.drafted[first + j] == t;
+      }
+    }
+    const float y = lg_used(static_cast<float>(x.in[t]), times > 0 || (what & LG_PROMPT), times, rep, freq, pres, a.list_bias[room + i]);
+    x.out[t] = static_cast<T>(y);
+  }
+}
+
+// Where the lists of a call lie in its workspace, and how large that is.
+static long lg_lists(LogitsArgs& a, void* work) {
+  a.bucket_shift = 12;
+  while (((a.vocab - 1) >> a.bucket_shift) + 1 > LG_BUCKETS) ++a.bucket_shift;
+  const int buckets = ((a.vocab - 1) >> a.bucket_shift) + 1;
+  const long listed = static_cast<long>(a.penal ? a.text + (a.cu != nullptr ? TREE_MAX : 0) : 0) + a.biases;
+  a.list_room = listed < a.vocab ? listed : a.vocab;
+  char* at = static_cast<char*>(work);
+  auto take = [&](long bytes) {
+    char* was = at;
+    at += (bytes + 15) / 16 * 16;
+    return was;
+  };
+  const long S = a.requests;
+  a.row_way = reinterpret_cast<uint4*>(take(a.cu != nullptr ? a.rows * 16l : 0));
+  a.row_request = reinterpret_cast<int*>(take(a.cu != nullptr ? a.rows * 4l : 0));
+  a.list_start = reinterpret_cast<int*>(take(S * (buckets + 1) * 4));
+  a.list_token = reinterpret_cast<int*>(take(S * a.list_room * 4));
+  a.list_what = reinterpret_cast<int*>(take(S * a.list_room * 4));
+  a.list_bias = reinterpret_cast<float*>(take(S * a.list_room * 4));
+  return at - static_cast<char*>(work);
+}
+
+// Small calls: everything in one launch, 8 tokens a thread.
+static bool lg_small(const LogitsArgs& a, int sms) { return static_cast<long>((a.vocab + 7 + 2047) / 2048) * a.rows <= 8L * sms; }
+
+template <int HASH>
+static cudaError_t launch_count(const LogitsArgs& a, cudaStream_t s) {
+  auto kern = logits_count_kernel<HASH>;
+  if (cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), 2 * HASH * 4); e != cudaSuccess) return e;
+  return launch_pdl(kern, dim3(a.requests), dim3(HASH / 16), 2 * HASH * 4, s, a);
 }
 
 template <typename T>
-static int launch_logits(LogitsArgs a, int sms, cudaStream_t s) {
-  constexpr int E = 16 / sizeof(T), SMALL = 2048, LARGE = 4 * E * LG_THREADS;
+static int launch_logits(LogitsArgs a, void* work, long work_bytes, int sms, cudaStream_t s) {
+  constexpr int E = 16 / sizeof(T), CHUNK = 4 * E * LG_THREADS;
   auto chunks_of = [&](int chunk) { return (a.vocab + E - 1 + chunk - 1) / chunk; };  // (a row may start up to E - 1 places into its first 16 bytes)
-  const bool used = a.penal || a.biases > 0;
-  if (used && static_cast<long>(chunks_of(SMALL)) * a.rows <= 8L * sms) {
-    a.chunks = chunks_of(SMALL);
-    return (int)launch_pdl(logits_kernel<T, SMALL>, dim3(a.chunks * a.rows), dim3(LG_THREADS), 0, s, a);
+  if (a.penal || a.biases > 0) {
+    if (lg_small(a, sms)) {
+      a.chunks = chunks_of(2048);
+      return (int)launch_pdl(logits_kernel<T, 2048>, dim3(a.chunks * a.rows), dim3(LG_THREADS), 0, s, a);
+    }
+    if (lg_lists(a, work) > work_bytes) return (int)cudaErrorInvalidValue;
+    // 64 KB of table leave room for three CTAs on an SM, 128 KB take a text of 12,000 tokens
+    const cudaError_t e = static_cast<long>(a.text) + a.biases + TREE_MAX <= 6144 ? launch_count<8192>(a, s) : launch_count<16384>(a, s);
+    if (e != cudaSuccess) return (int)e;
+    a.listed = 1;
   }
-  if (a.allowed != nullptr || a.in != a.out || a.in_row != a.out_row) {
-    a.chunks = chunks_of(LARGE);
-    const long ctas = static_cast<long>(a.chunks) * a.rows;
-    if (ctas > 0x7fffffffl) return (int)cudaErrorInvalidValue;
-    if (cudaError_t e = launch_pdl(logits_mask_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(LG_THREADS), 0, s, a); e != cudaSuccess) return (int)e;
-    a.behind_mask = 1;
-  }
-  if (!used) return 0;
-  // 64 KB of table leave room for three CTAs on an SM, 128 KB take a text of 12,000 tokens
-  return static_cast<long>(a.text) + a.biases + TREE_MAX <= 6144 ? launch_used<T, 8192>(a, sms, s) : launch_used<T, 16384>(a, sms, s);
+  a.chunks = chunks_of(CHUNK);
+  const long ctas = static_cast<long>(a.chunks) * a.rows;
+  if (ctas > 0x7fffffffl) return (int)cudaErrorInvalidValue;
+  return (int)launch_pdl(logits_row_kernel<T>, dim3(static_cast<unsigned>(ctas)), dim3(LG_THREADS), 0, s, a);
 }
 
 }  // namespace sb
 
 // call: addresses of in, out, tokens, lengths, prompts, repetition, frequency, presence, bias ids, bias values, allowed, drafted, parents, cu (null: not there); then
 // the pitches of in, out, tokens, biases and allowed (elements), rows, requests, vocabulary, tokens of a text, biases of a request, whether in and
-// out are fp32 (else bf16), SMs. in and out may be the same. Tokens outside the vocabulary (of texts, trees and biases) count for nothing. With trees, row r is
+// out are fp32 (else bf16), SMs, address
+// and bytes of a workspace of the size that sb_adjust_logits_work names. in and out may be the same. Tokens outside the vocabulary (of texts, trees and biases) count for nothing. With trees, row r is
 // node r - cu[b] of tree b; rows behind cu[requests] are left as they are.
 extern "C" int sb_adjust_logits(const void* call, cudaStream_t s) {
   const long long* x = static_cast<const long long*>(call);
@@ -522,5 +546,21 @@ extern "C" int sb_adjust_logits(const void* call, cudaStream_t s) {
   if (a.rows <= 0 || a.vocab <= 0) return 0;
   a.penal = a.repetition != nullptr || a.frequency != nullptr || a.presence != nullptr;
   const int sms = static_cast<int>(x[25]);
-  return x[24] ? sb::launch_logits<float>(a, sms, s) : sb::launch_logits<__nv_bfloat16>(a, sms, s);
+  void* work = reinterpret_cast<void*>(x[26]);
+  return x[24] ? sb::launch_logits<float>(a, work, x[27], sms, s) : sb::launch_logits<__nv_bfloat16>(a, work, x[27], sms, s);
+}
+
+// Bytes of workspace of a call with so many rows, requests, tokens of vocabulary and of a text (0: no penalties) and biases; 0: it needs none.
+extern "C" int sb_adjust_logits_work(int rows, int requests, int vocab, int text, int biases, int penal, int tree, int sms, long* bytes) {
+  static const int some = 0;
+  sb::LogitsArgs a = {};
+  a.rows = rows;
+  a.requests = requests;
+  a.vocab = vocab;
+  a.text = text;
+  a.biases = biases;
+  a.penal = penal;
+  a.cu = tree ? &some : nullptr;
+  *bytes = (penal || biases > 0) && rows > 0 && vocab > 0 && !sb::lg_small(a, sms) ? sb::lg_lists(a, nullptr) : 0;
+  return 0;
 }

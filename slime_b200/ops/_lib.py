@@ -96,6 +96,7 @@ _SIGS = {
     "sb_sample": [P, I, L, I, I, P, P, P, P, P, P, P, P, P, P, I, P],
     "sb_tree_attn": [P] * 9 + [I] * 9 + [L] * 7 + [F, I, P],
     "sb_adjust_logits": [P, P],
+    "sb_adjust_logits_work": [I, I, I, I, I, I, I, I, P],
     "sb_tree_attn_plan": [I, I, I, I, I, L, I, I, P],
     "sb_tree_attn_tc": [P, F, P],
     "sb_tree_accept": [P, P],

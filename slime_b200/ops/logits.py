@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import struct
 
 import torch
@@ -9,7 +11,15 @@ import torch
 from slime_b200.ops import _checks, _lib, reference, tree as _tree
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
-_CALL = struct.Struct("26q").pack  # arguments of the C entry
+_CALL = struct.Struct("28q").pack  # arguments of the C entry
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace(rows: int, requests: int, vocab: int, text: int, biases: int, penal: bool, tree: bool, sms: int) -> int:
+    """Bytes of workspace of a call."""
+    size = ctypes.c_long()
+    _lib.check(_lib.lib().sb_adjust_logits_work(rows, requests, vocab, text, biases, penal, tree, sms, ctypes.byref(size)), "sb_adjust_logits_work", 0)
+    return size.value
 
 
 def _per_request(op: str, name: str, t, requests: int, device):
@@ -78,10 +88,13 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     K = 0 if bias_ids is None else bias_ids.shape[1]
     text, pitch = (tokens.shape[1], tokens.stride(0)) if penal else (0, 0)
+    sms = _tree._facts(dev)[0]
+    size = _workspace(R, S, V, text, K, penal, tree is not None, sms) if penal or K else 0
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     rc = _lib.lib().sb_adjust_logits(
         _CALL(logits.data_ptr(), out.data_ptr(), at(tokens), at(lengths), at(prompt_lens), at(repetition), at(frequency), at(presence), at(bias_ids),
               at(bias_values), at(allowed), at(drafted), at(parents), at(cu_nodes), logits.stride(0), out.stride(0), pitch, K,
-              0 if allowed is None else allowed.stride(0), R, S, V, text, K, dtype is _F32, _tree._facts(dev)[0]), _lib.stream())  # fmt: skip
+              0 if allowed is None else allowed.stride(0), R, S, V, text, K, dtype is _F32, sms, at(work), size), _lib.stream())  # fmt: skip
     _lib.check(rc, "sb_adjust_logits")
     return out
 
