@@ -125,18 +125,15 @@ template <typename F>
 __device__ __forceinline__ void lg_text(const LogitsArgs& a, int req, int threads, const F& each) {
   const int* text = a.tokens + req * a.tokens_row;
   const int len = max(min(a.lengths[req], a.text), 0);
-  int from = 0;
-  if ((reinterpret_cast<uintptr_t>(text) & 15) == 0) {
-    from = len & ~3;
-    for (int i = 4 * threadIdx.x; i < from; i += 4 * threads) {
-      const int4 t = *reinterpret_cast<const int4*>(text + i);
-      each(i, t.x);
-      each(i + 1, t.y);
-      each(i + 2, t.z);
-      each(i + 3, t.w);
-    }
+  constexpr int FLY = 8;  // tokens whose reads are under way together
+  for (int i0 = threadIdx.x; i0 < len; i0 += FLY * threads) {
+    int t[FLY];
+#pragma unroll
+    for (int x = 0; x < FLY; ++x) t[x] = i0 + x * threads < len ? text[i0 + x * threads] : -1;
+#pragma unroll
+    for (int x = 0; x < FLY; ++x)
+      if (i0 + x * threads < len) each(i0 + x * threads, t[x]);
   }
-  for (int i = from + threadIdx.x; i < len; i += threads) each(i, text[i]);
 }
 
 // ---------------------------------------------------------------- one launch: CHUNK tokens of a row, CHUNK / 256 a thread
@@ -331,7 +328,7 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
         ++at;
       }
     };
-    uint32_t brought = 0, brought_x = 0;  // of this thread's tokens of the text, one bit each (at most 17); of drafted nodes and biases
+    uint32_t brought = 0, brought_x = 0;  // of this thread's tokens of the text, one bit each (at most 12); of drafted nodes and biases
     bool came;
     if (counts) {
       int x = 0;
