@@ -40,14 +40,13 @@ struct LogitsArgs {
   int penal;
   // what logits_count_kernel leaves for logits_row_kernel: of each row of a tree the nodes on its way and its request; of each request the tokens
   // to work out, what there is of them and their biases, by bucket of 2^bucket_shift tokens
-  int listed, bucket_shift;
+  int listed, bucket_shift, lists;  // lists of a request: token t is in list t % lists
   long list_room;
   uint4* row_way;
   int* row_request;
-  int* list_start;        // [S, buckets + 1]
-  int* list_token;        // [S, list_room]
-  int* list_what;
-  float* list_bias;
+  int* list_start;        // [S, lists, buckets + 1]
+  int2* list;             // [S, lists, list_room] token, what there is of it
+  float* list_bias;       // where it has a bias
 };
 
 // 16-byte pieces of a row. A row's places are numbered from the 16-byte boundary at or in front of its start, so that place p is token p - off.
@@ -121,18 +120,19 @@ __device__ __forceinline__ float lg_used(float v, bool seen, int times, float re
 
 // What there is of a token: in the prompt, has a bias, was drafted, and how many times it was answered with. lg_text: each token of a request's text.
 enum : int { LG_PROMPT = 1 << 30, LG_BIAS = 1 << 29, LG_DRAFT = 1 << 28 };
+constexpr int LG_FLY = 8;  // tokens whose reads are under way together
 template <typename F>
 __device__ __forceinline__ void lg_text(const LogitsArgs& a, int req, int threads, const F& each) {
   const int* text = a.tokens + req * a.tokens_row;
   const int len = max(min(a.lengths[req], a.text), 0);
-  constexpr int FLY = 8;  // tokens whose reads are under way together
-  for (int i0 = threadIdx.x; i0 < len; i0 += FLY * threads) {
-    int t[FLY];
+  for (int i0 = threadIdx.x; i0 < len; i0 += LG_FLY * threads) {
+    int t[LG_FLY];  // tokens at i0 + x threads; -1: none (or one outside the vocabulary)
 #pragma unroll
-    for (int x = 0; x < FLY; ++x) t[x] = i0 + x * threads < len ? text[i0 + x * threads] : -1;
-#pragma unroll
-    for (int x = 0; x < FLY; ++x)
-      if (i0 + x * threads < len) each(i0 + x * threads, t[x]);
+    for (int x = 0; x < LG_FLY; ++x) {
+      t[x] = i0 + x * threads < len ? text[i0 + x * threads] : -1;
+      if (static_cast<unsigned>(t[x]) >= static_cast<unsigned>(a.vocab)) t[x] = -1;
+    }
+    each(i0, t);
   }
 }
 
@@ -184,11 +184,13 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
   __syncthreads();
   if (counts) {
     const int prompt = a.prompts != nullptr ? a.prompts[req] : 0;
-    lg_text(a, req, LG_THREADS, [&](int i, int t) {
-      if (const int at = place(t); at >= 0) {
-        if (i < prompt) atomicOr(&count[at], LG_PROMPT);
-        else atomicAdd(&count[at], 1);
-      }
+    lg_text(a, req, LG_THREADS, [&](int i0, const int (&t)[LG_FLY]) {
+#pragma unroll
+      for (int x = 0; x < LG_FLY; ++x)
+        if (const int at = place(t[x]); at >= 0) {
+          if (i0 + x * LG_THREADS < prompt) atomicOr(&count[at], LG_PROMPT);
+          else atomicAdd(&count[at], 1);
+        }
     });
     if (r - first < n) {  // the drafted tokens on the way to this row
       uint32_t set[4];
@@ -255,7 +257,7 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
 // Lists the tokens of a request that were used, drafted or have a bias, by bucket of the vocabulary. They are counted in a hash table of HASH places
 // in shared memory (linear probing, at most three quarters full); a longer text is counted in a table of 2 HASH tokens of the vocabulary at a time.
 template <int HASH>
-__global__ void __launch_bounds__(HASH / 16, HASH == 8192 ? 3 : 1)
+__global__ void __launch_bounds__(HASH / 16, HASH == 8192 ? 2 : 1)
 logits_count_kernel(const __grid_constant__ LogitsArgs a) {
   constexpr int THREADS = HASH / 16;
   extern __shared__ __align__(16) int tables[];
@@ -265,7 +267,7 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
   __shared__ int start[LG_BUCKETS + 1];  // places in the list: how many of a bucket, then where the next one goes
   __shared__ int sums[32];
   pdl_wait();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, req = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, req = blockIdx.x / a.lists, part = blockIdx.x - req * a.lists;
   int first = 0, until = 0, n = 0;
   if (a.cu != nullptr) {
     first = a.cu[req];
@@ -287,7 +289,7 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
     tree_t[i] = a.drafted[first + i];
   }
   __syncthreads();
-  if (first >= 0)
+  if (first >= 0 && part == 0)
     for (int r = first + tid; r < until; r += THREADS) {  // rows of the tree: whose they are, and the nodes on the way to them (the root is the text's last token)
       uint32_t set[4] = {0, 0, 0, 0};
       if (r - first < n) tree_way_up([&](int j) { return tree_p[j]; }, r - first, set);
@@ -295,10 +297,10 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
       a.row_request[r] = req;
     }
   const int buckets = ((a.vocab - 1) >> a.bucket_shift) + 1;
-  int* list_start = a.list_start + static_cast<long>(req) * (buckets + 1);
-  int* list_token = a.list_token + static_cast<long>(req) * a.list_room;
-  int* list_what = a.list_what + static_cast<long>(req) * a.list_room;
-  float* list_bias = a.list_bias + static_cast<long>(req) * a.list_room;
+  int* list_start = a.list_start + static_cast<long>(blockIdx.x) * (buckets + 1);
+  int2* list = a.list + static_cast<long>(blockIdx.x) * a.list_room;
+  float* list_bias = a.list_bias + static_cast<long>(blockIdx.x) * a.list_room;
+  auto ours = [&](int t) { return static_cast<unsigned>(t) < static_cast<unsigned>(a.vocab) && (t & (a.lists - 1)) == part; };
   const int passes = direct ? (a.vocab + 2 * HASH - 1) / (2 * HASH) : 1;
   for (int i = tid; i < buckets; i += THREADS) start[i] = 0;
   int listed = 0;  // by the passes before
@@ -311,34 +313,65 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
     }
     __syncthreads();
     // ---- what there is of each token. came: it was not there before; in the hash table the thread that brought it lists it
-    auto place = [&](int t, bool& came) -> int* {
+    auto hash = [&](int t) { return static_cast<int>((static_cast<unsigned>(t) * 2654435761u) >> 16) & (HASH - 1); };  // Knuth's multiplicative hashing
+    auto look = [&](int at) { return *static_cast<volatile int*>(&keys[at]); };
+    auto probe = [&](int t, int at, bool& came) -> int {  // the place of t, from place `at` on
       came = false;
-      if (static_cast<unsigned>(t) >= static_cast<unsigned>(a.vocab)) return nullptr;
-      if (direct) return t >= base && t - base < 2 * HASH ? tables + (t - base) : nullptr;
-      unsigned at = (static_cast<unsigned>(t) * 2654435761u) >> 16;  // Knuth's multiplicative hashing
       while (true) {
-        at &= HASH - 1;
-        int was = *static_cast<volatile int*>(&keys[at]);
+        int was = look(at);
         if (was == -1) {
           was = atomicCAS(&keys[at], -1, t);
           came = was == -1;
           if (came) atomicAdd(&start[t >> a.bucket_shift], 1);
         }
-        if (was == -1 || was == t) return &hashed[at];
-        ++at;
+        if (was == -1 || was == t) return at;
+        at = (at + 1) & (HASH - 1);
       }
     };
-    uint32_t brought = 0, brought_x = 0;  // of this thread's tokens of the text, one bit each (at most 12); of drafted nodes and biases
+    auto place = [&](int t, bool& came) -> int* {
+      came = false;
+      if (!ours(t)) return nullptr;
+      if (direct) return t >= base && t - base < 2 * HASH ? tables + (t - base) : nullptr;
+      return &hashed[probe(t, hash(t), came)];
+    };
+    uint32_t brought = 0, brought_x = 0;  // of this thread's tokens of the text, one bit each (at most 16); of drafted nodes and biases
     bool came;
     if (counts) {
-      int x = 0;
-      lg_text(a, req, THREADS, [&](int i, int t) {
-        if (int* at = place(t, came); at != nullptr) {
-          if (i < prompt) atomicOr(at, LG_PROMPT);
-          else atomicAdd(at, 1);
-          if (came) brought |= 1u << (x & 31);
+      int batch = 0;
+      lg_text(a, req, THREADS, [&](int i0, const int (&t)[LG_FLY]) {
+        // a step for all tokens at a time: nearly all of them are found, or find an empty place, at the first look
+        int at[LG_FLY], was[LG_FLY];
+        if (!direct) {
+#pragma unroll
+          for (int x = 0; x < LG_FLY; ++x) {
+            at[x] = hash(t[x]);
+            was[x] = ours(t[x]) ? look(at[x]) : -1;
+          }
+#pragma unroll
+          for (int x = 0; x < LG_FLY; ++x)
+            if (ours(t[x]) && was[x] == -1) {
+              was[x] = atomicCAS(&keys[at[x]], -1, t[x]);
+              if (was[x] == -1) {
+                was[x] = t[x];
+                brought |= 1u << (batch * LG_FLY + x);
+                atomicAdd(&start[t[x] >> a.bucket_shift], 1);
+              }
+            }
+#pragma unroll
+          for (int x = 0; x < LG_FLY; ++x)
+            if (ours(t[x]) && was[x] != t[x]) {
+              at[x] = probe(t[x], at[x], came);
+              if (came) brought |= 1u << (batch * LG_FLY + x);
+            }
         }
-        ++x;
+#pragma unroll
+        for (int x = 0; x < LG_FLY; ++x) {
+          if (!ours(t[x]) || (direct && (t[x] < base || t[x] - base >= 2 * HASH))) continue;
+          int* what = direct ? tables + (t[x] - base) : hashed + at[x];
+          if (i0 + x * THREADS < prompt) atomicOr(what, LG_PROMPT);
+          else atomicAdd(what, 1);
+        }
+        batch = min(batch + 1, 3);  // (more than two batches: the direct table, which needs no marks)
       });
       if (tid > 0 && tid < n)
         if (int* at = place(tree_t[tid], came); at != nullptr) {
@@ -386,23 +419,33 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
     if (pass + 1 == passes && tid == 0) list_start[buckets] = listed;
     auto put = [&](int t, int what, float bias) {
       const int at = atomicAdd(&start[t >> a.bucket_shift], 1);
-      list_token[at] = t;
-      list_what[at] = what;
-      list_bias[at] = bias;
+      list[at] = make_int2(t, what);
+      if (what & LG_BIAS) list_bias[at] = bias;
     };
     if (direct) {
       for (int at = tid; at < 2 * HASH; at += THREADS)
         if (const int what = tables[at]; what != 0 && (what & LG_BIAS) == 0) put(base + at, what, 0.f);
     } else if (counts) {
-      auto list = [&](int t) {
-        if (const int what = *place(t, came); (what & LG_BIAS) == 0) put(t, what, 0.f);
-      };
-      int x = 0;
-      lg_text(a, req, THREADS, [&](int, int t) {
-        if (brought >> (x & 31) & 1) list(t);
-        ++x;
+      int batch = 0;
+      lg_text(a, req, THREADS, [&](int, const int (&t)[LG_FLY]) {
+        const uint32_t own = brought >> (batch++ * LG_FLY);
+        int at[LG_FLY], to[LG_FLY], what[LG_FLY];
+#pragma unroll
+        for (int x = 0; x < LG_FLY; ++x) at[x] = own >> x & 1 ? hash(t[x]) : -1;
+#pragma unroll
+        for (int x = 0; x < LG_FLY; ++x)
+          while (at[x] >= 0 && look(at[x]) != t[x]) at[x] = (at[x] + 1) & (HASH - 1);
+#pragma unroll
+        for (int x = 0; x < LG_FLY; ++x) {
+          what[x] = at[x] >= 0 ? hashed[at[x]] : LG_BIAS;
+          to[x] = (what[x] & LG_BIAS) == 0 ? atomicAdd(&start[t[x] >> a.bucket_shift], 1) : -1;
+        }
+#pragma unroll
+        for (int x = 0; x < LG_FLY; ++x)
+          if (to[x] >= 0) list[to[x]] = make_int2(t[x], what[x]);
       });
-      if (brought_x) list(tree_t[tid]);
+      if (brought_x)
+        if (const int what = *place(tree_t[tid], came); (what & LG_BIAS) == 0) put(tree_t[tid], what, 0.f);
     }
     for (int i = tid, x = 0; i < K; i += THREADS, ++x) {
       const int id = ids[i];
@@ -443,15 +486,18 @@ logits_row_kernel(const __grid_constant__ LogitsArgs a) {
   if (a.listed) pdl_wait();
   pdl_launch_dependents();
   const int lo = max(x.base, 0), hi = min(x.base + CHUNK, a.vocab);  // the chunk's tokens
+  // the request's lists share the threads
   int req = r, from = 0, until = 0;
-  long room = 0;
+  const int share = LG_THREADS / max(a.lists, 1), mine = tid / share;
+  long at = 0;
   if (a.listed && lo < hi) {
     if (a.cu != nullptr) req = a.row_request[r];
     const int buckets = ((a.vocab - 1) >> a.bucket_shift) + 1;
-    const int* list_start = a.list_start + static_cast<long>(req) * (buckets + 1);
+    at = static_cast<long>(req) * a.lists + mine;
+    const int* list_start = a.list_start + at * (buckets + 1);
     from = list_start[lo >> a.bucket_shift];
     until = list_start[((hi - 1) >> a.bucket_shift) + 1];
-    room = static_cast<long>(req) * a.list_room;
+    at *= a.list_room;
   }
   const bool in_place = a.in == a.out && a.in_row == a.out_row;
 #pragma unroll
@@ -467,13 +513,15 @@ logits_row_kernel(const __grid_constant__ LogitsArgs a) {
     }
     x.store(a, i);
   }
-  if (from >= until) return;
+  if (!a.listed) return;
   __syncthreads();
+  if (from >= until) return;
   const float rep = a.repetition != nullptr ? a.repetition[req] : 1.f;
   const float freq = a.frequency != nullptr ? a.frequency[req] : 0.f;
   const float pres = a.presence != nullptr ? a.presence[req] : 0.f;
-  for (int i = from + tid; i < until; i += LG_THREADS) {
-    const int t = a.list_token[room + i], what = a.list_what[room + i];
+  for (int i = from + tid - mine * share; i < until; i += share) {
+    const int2 entry = a.list[at + i];
+    const int t = entry.x, what = entry.y;
     if (t < lo || t >= hi) continue;
     if (a.allowed != nullptr && (a.allowed[r * a.allowed_row + (t >> 5)] >> (t & 31) & 1) == 0) continue;  // (hidden: -infinity already)
     int times = what & (LG_DRAFT - 1);
@@ -485,14 +533,14 @@ logits_row_kernel(const __grid_constant__ LogitsArgs a) {
         if (word >> (j & 31) & 1) times += a.drafted[first + j] == t;
       }
     }
-    const float y = lg_used(static_cast<float>(x.in[t]), times > 0 || (what & LG_PROMPT), times, rep, freq, pres, a.list_bias[room + i]);
+    const float y = lg_used(static_cast<float>(x.in[t]), times > 0 || (what & LG_PROMPT), times, rep, freq, pres, what & LG_BIAS ? a.list_bias[at + i] : 0.f);
     x.out[t] = static_cast<T>(y);
   }
 }
 
 // Where the lists of a call lie in its workspace, and how large that is.
-static long lg_lists(LogitsArgs& a, void* work) {
-  a.bucket_shift = 12;
+static long lg_lists(LogitsArgs& a, void* work, int sms) {
+  a.bucket_shift = 8;  // (few tokens share a bucket, and with it a counter)
   while (((a.vocab - 1) >> a.bucket_shift) + 1 > LG_BUCKETS) ++a.bucket_shift;
   const int buckets = ((a.vocab - 1) >> a.bucket_shift) + 1;
   const long listed = static_cast<long>(a.penal ? a.text + (a.cu != nullptr ? TREE_MAX : 0) : 0) + a.biases;
@@ -503,13 +551,15 @@ static long lg_lists(LogitsArgs& a, void* work) {
     at += (bytes + 15) / 16 * 16;
     return was;
   };
-  const long S = a.requests;
+  // few requests: several CTAs count each, every one some of the tokens (by their lowest bits) for a list of its own
+  a.lists = 1;
+  while (a.lists < 8 && static_cast<long>(a.requests) * a.lists * 2 <= 2l * sms) a.lists *= 2;
+  const long S = static_cast<long>(a.requests) * a.lists;
   a.row_way = reinterpret_cast<uint4*>(take(a.cu != nullptr ? a.rows * 16l : 0));
   a.row_request = reinterpret_cast<int*>(take(a.cu != nullptr ? a.rows * 4l : 0));
   a.list_start = reinterpret_cast<int*>(take(S * (buckets + 1) * 4));
-  a.list_token = reinterpret_cast<int*>(take(S * a.list_room * 4));
-  a.list_what = reinterpret_cast<int*>(take(S * a.list_room * 4));
-  a.list_bias = reinterpret_cast<float*>(take(S * a.list_room * 4));
+  a.list = reinterpret_cast<int2*>(take(S * a.list_room * 8));
+  a.list_bias = reinterpret_cast<float*>(take(a.biases > 0 ? S * a.list_room * 4 : 0));
   return at - static_cast<char*>(work);
 }
 
@@ -520,7 +570,7 @@ template <int HASH>
 static cudaError_t launch_count(const LogitsArgs& a, cudaStream_t s) {
   auto kern = logits_count_kernel<HASH>;
   if (cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), 2 * HASH * 4); e != cudaSuccess) return e;
-  return launch_pdl(kern, dim3(a.requests), dim3(HASH / 16), 2 * HASH * 4, s, a);
+  return launch_pdl(kern, dim3(a.requests * a.lists), dim3(HASH / 16), 2 * HASH * 4, s, a);
 }
 
 template <typename T>
@@ -532,7 +582,7 @@ static int launch_logits(LogitsArgs a, void* work, long work_bytes, int sms, cud
       a.chunks = chunks_of(2048);
       return (int)launch_pdl(logits_kernel<T, 2048>, dim3(a.chunks * a.rows), dim3(LG_THREADS), 0, s, a);
     }
-    if (lg_lists(a, work) > work_bytes) return (int)cudaErrorInvalidValue;
+    if (lg_lists(a, work, sms) > work_bytes) return (int)cudaErrorInvalidValue;
     // 64 KB of table leave room for three CTAs on an SM, 128 KB take a text of 12,000 tokens
     const cudaError_t e = static_cast<long>(a.text) + a.biases + TREE_MAX <= 6144 ? launch_count<8192>(a, s) : launch_count<16384>(a, s);
     if (e != cudaSuccess) return (int)e;
@@ -583,6 +633,6 @@ extern "C" int sb_adjust_logits_work(int rows, int requests, int vocab, int text
   a.biases = biases;
   a.penal = penal;
   a.cu = tree ? &some : nullptr;
-  *bytes = (penal || biases > 0) && rows > 0 && vocab > 0 && !sb::lg_small(a, sms) ? sb::lg_lists(a, nullptr) : 0;
+  *bytes = (penal || biases > 0) && rows > 0 && vocab > 0 && !sb::lg_small(a, sms) ? sb::lg_lists(a, nullptr, sms) : 0;
   return 0;
 }
