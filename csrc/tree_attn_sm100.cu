@@ -5,7 +5,8 @@
 // query tile (row = node * G + head), so 128-key tiles come in once for up to 128 rows, or 256 where a tree has more.
 //
 //   S_g  = Q K_j^T            M 128, N 128, K D       TMEM
-//   P_g  = 2^(S_g c - m)      TMEM -> registers -> bf16 over the scores it came from (the A operand of the next product)
+//   P_g  = 2^(S_g c - m)      TMEM -> registers -> bf16 in TMEM (the A operand of the next product): with heads of 64 beside the scores it came from, so
+//                             that the next scores run beside this softmax; with heads of 128 there is room only over them
 //   O_g += P_g V_j            M 128, N D, K 128       TMEM
 //
 // One CTA per SM: warps 0 and 3 issue TMA loads (a box per page and 64-wide chunk), warps 1 and 2 the products of one group each, and two
@@ -49,7 +50,9 @@ struct TtSmem {
   // behind the ring: ways up [2 pieces][128 nodes], (m, l) [2 pieces][2 groups][128 rows], parents [128], requests, barriers
   static constexpr int EXTRA = 2 * 128 * 16 + 2 * 2 * 128 * 8 + 128 * 4 + RED + TABLE + 512;
   static constexpr int TOTAL = TILES * Q_TILE + RING * KV_TILE + EXTRA + 1024;  // +1024: alignment
-  static constexpr int TMEM_COLS = 512;              // S_0 @0, S_1 @128, O_0 @256, O_1 @256 + D
+  static constexpr int TMEM_COLS = 512;              // S_0 @0, S_1 @128, O_0 @256, O_1 @256 + D, and with heads of 64 P_0 @384, P_1 @448
+  static constexpr bool APART = D == 64;             // P beside its scores, not over them: the next scores need not wait for the product
+  static constexpr int P_COL = APART ? 384 : 0, P_STEP = APART ? 64 : TT_BN;
 };
 
 __device__ __forceinline__ float tt_exp2(float x) {
@@ -169,7 +172,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   uint64_t* w_full = o_empty + 1;      // [2] ways of the piece are there
   uint64_t* w_empty = w_full + 2;      // [2] ... and have been used (8 arrivals)
   uint64_t* my_turn = w_empty + 2;     // [2] the other group's issuer is done with its step
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(my_turn + 2);
+  uint64_t* s_free = my_turn + 2;      // [2] P apart: the group has read its scores (4 arrivals)
+  uint64_t* o_step = s_free + 2;       // [2] P apart: the group's product is done, P may be written again
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_step + 2);
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 2);  // [0] request, [1] unit within it
   int* sums = start + 2;                               // [12] units of the warps' requests
@@ -188,6 +193,8 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       mbar_init(&w_full[g], 1);
       mbar_init(&w_empty[g], 8);
       mbar_init(&my_turn[g], 1);
+      mbar_init(&s_free[g], 4);
+      mbar_init(&o_step[g], 1);
     }
     mbar_init(o_empty, 8);
     *cta_abort = 0;
@@ -363,7 +370,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       };
       struct Group {
         TtWalk<TILES> walk;
-        uint32_t t0, turn, piece, steps;  // tiles and turns of the pieces before, pieces, products so far
+        uint32_t t0, turn, piece;  // tiles and turns of the pieces before, pieces
         int i;                            // the next scores: the group's i-th step of the piece
         bool more;
         // the step whose scores are issued
@@ -419,43 +426,51 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           s.more = s.walk.next(a);
         }
       };
-      auto begin = [&](Group& s, int g) {
-        s = {};
-        s.walk = walk;
-        s.more = s.walk.next(a);
-        scores(s, g);
+      constexpr bool TURNS = TILES == 2 && !S::APART;
+      struct Step {
+        uint32_t tile, of_piece;
+        bool first, last, rows2;
       };
-      auto step = [&](Group& s, int g) -> bool {
-        if (!ok || !s.there) return false;
-        wait(&p_full[g], s.steps++ & 1, ERR_WAIT_TMEM_EMPTY);
-        const uint32_t vs = s.tile % S::V_RING;
-        wait(&full[S::K_RING + s.tile % S::V_FULL], s.tile / S::V_FULL & 1, ERR_WAIT_FULL);
-        if (s.first) wait(o_empty, (s.of_piece & 1) ^ 1, ERR_WAIT_TMEM_EMPTY);  // (the accumulators of the last piece have been read)
-        if (TILES == 2) wait(&my_turn[g], (s.steps - 1) & 1, ERR_WAIT_EMPTY);
-        if (!ok) return false;
+      auto product = [&](const Step& x, uint32_t steps, int g) {
+        wait(&p_full[g], steps & 1, ERR_WAIT_TMEM_EMPTY);
+        if (x.first) wait(o_empty, (x.of_piece & 1) ^ 1, ERR_WAIT_TMEM_EMPTY);  // (the accumulators of the last piece have been read)
+        const uint32_t vs = x.tile % S::V_RING;
+        wait(&full[S::K_RING + x.tile % S::V_FULL], x.tile / S::V_FULL & 1, ERR_WAIT_FULL);
+        if (TURNS) wait(&my_turn[g], steps & 1, ERR_WAIT_EMPTY);
+        if (!ok) return;
         tc_fence_after();
         const uint64_t vd = v_desc + (S::K_RING + uniform(vs)) * (S::KV_TILE >> 4);
-        const uint32_t more_o = uniform(s.first ? 0u : 1u), d_o = tmem + 2 * TT_BN + uniform(g) * D, a_o = tmem + uniform(g) * TT_BN;
+        const uint32_t more_o = uniform(x.first ? 0u : 1u), d_o = tmem + 2 * TT_BN + uniform(g) * D, a_o = tmem + S::P_COL + uniform(g) * S::P_STEP;
         if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < TT_BN / 16; ++k)
-            umma_f16_ts(d_o, a_o + k * 8, vd + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more_o);
+          for (int k = 0; k < TT_BN / 16; ++k) umma_f16_ts(d_o, a_o + k * 8, vd + k * (2048 >> 4), idesc_o, k != 0 ? 1u : more_o);
           umma_commit(&empty[S::K_RING + vs]);
-          if (!s.rows2) mbar_arrive(&empty[S::K_RING + vs]);
-          if (s.last) umma_commit(&o_full[g]);
+          if (!x.rows2) mbar_arrive(&empty[S::K_RING + vs]);
+          if (S::APART) umma_commit(&o_step[g]);
+          if (x.last) umma_commit(&o_full[g]);
         }
         __syncwarp();
-        scores(s, g);
-        if (TILES == 2 && elect_one()) mbar_arrive(&my_turn[g ^ 1]);
-        __syncwarp();
-        return ok;
       };
       const int g = warp - 1;
-      if (TILES == 2 && g == 1 && elect_one()) mbar_arrive(&my_turn[0]);  // group 0 begins
+      if (TURNS && g == 1 && elect_one()) mbar_arrive(&my_turn[0]);  // group 0 begins
       __syncwarp();
-      Group s;
-      begin(s, g);
-      while (step(s, g)) {
+      Group s = {};
+      s.walk = walk;
+      s.more = s.walk.next(a);
+      scores(s, g);
+      for (uint32_t steps = 0; ok && s.there; ++steps) {
+        const Step x = {s.tile, s.of_piece, s.first, s.last, s.rows2};
+        if (S::APART && !x.last) {  // the next scores run beside this step's softmax
+          wait(&s_free[g], steps & 1, ERR_WAIT_TMEM_EMPTY);
+          if (ok) scores(s, g);
+          if (ok) product(x, steps, g);
+        } else {  // (a piece's last product does not wait for the queries of the next)
+          product(x, steps, g);
+          if (S::APART) wait(&s_free[g], steps & 1, ERR_WAIT_TMEM_EMPTY);
+          if (ok) scores(s, g);
+        }
+        if (TURNS && elect_one()) mbar_arrive(&my_turn[g ^ 1]);
+        __syncwarp();
       }
     } else {
       // -------------------------------------------------------------------- softmax + epilogue
@@ -466,10 +481,16 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const int in_tile = rr / a.G, head_in = rr - in_tile * a.G;
       const int o_rr = tid / REP, o_in = o_rr / a.G, o_head = o_rr - o_in * a.G;  // the row that this thread adds up the copies of
       const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
-      const uint32_t s_addr = lane_addr + g * TT_BN, o_addr = lane_addr + 2 * TT_BN;
+      const uint32_t s_addr = lane_addr + g * TT_BN, o_addr = lane_addr + 2 * TT_BN, p_addr = lane_addr + S::P_COL + g * S::P_STEP;
       const uint64_t c2 = f2_pack(a.c_log2, a.c_log2);
       uint32_t t0 = 0, turn = 0, s_cnt = 0, o_cnt0 = 0, o_cnt1 = 0;
       bool ok = true;
+      if constexpr (REP > 1 && S::APART) {  // the other copies' weights: zero for good
+        const uint32_t none[16] = {};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) tmem_st_32x16(p_addr + x * 16, none);
+        tmem_st_wait();
+      }
       for (uint32_t piece = 0; walk.next(a); ++piece) {  // after an expired wait the threads still meet at the barriers
         const int nt = walk.nt, ctx = walk.r.ctx;
         const bool rows2 = TILES == 2 && walk.groups == 2;
@@ -499,6 +520,23 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (masked) {
             want_ways();
             if (!ok) break;
+          }
+          auto release = [&]() {  // P apart: the scores are in registers, the next ones may come
+            if (S::APART) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&s_free[g]);
+            }
+          };
+          bool settled = !S::APART || s_cnt + i == 0;
+          auto settle = [&]() {  // P apart: the group's last product is done, P and O may be written
+            if (!settled) ok = __all_sync(0xffffffffu, ok && tt_wait(&o_step[g], (s_cnt + i - 1) & 1, cta_abort, status, ERR_WAIT_TMEM_FULL));
+            settled = true;
+            tc_fence_after();
+          };
+          if (!active) {
+            release();
+            settle();
           }
           if (active) {
             // hides what the row does not see of columns [32 x, 32 x + 32) of this tile: it sees keys in front of the tree, and nodes on its way up
@@ -537,12 +575,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               }
               mx = fmaxf(mx, COLS > 32 ? fmaxf(top(ra), top(rb)) : top(ra));
             }
+            if constexpr (COLS < 128) release();
             mx *= a.c_log2;  // c > 0: the maximum commutes with the scaling
             const float m_new = fmaxf(m_run, mx);
             if (i == 0) {
               m_run = m_new;
             } else if (__any_sync(0xffffffffu, valid && m_new > m_run + 8.f)) {
-              // (the scores just read came after every earlier product, so O may be corrected)
+              // (with P over the scores, those just read came after every earlier product, so O may be corrected)
+              settle();
               const float f = m_new == -INFINITY ? 1.f : tt_exp2(m_run - m_new);
               l_run *= f;
 #pragma unroll 1
@@ -571,13 +611,14 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                 sum[(k >> 1) & 1] = f2_add(sum[(k >> 1) & 1], f2_pack(p0, p1));
                 pk[k >> 1] = pack_bf16x2(p0, p1);
               }
-              tmem_st_32x16(s_addr + x * 16, pk);
+              settle();
+              tmem_st_32x16(p_addr + x * 16, pk);
             };
-            if constexpr (REP > 1) {  // the other copies' columns
+            if constexpr (REP > 1 && !S::APART) {  // the other copies' columns
               const uint32_t none[16] = {};
 #pragma unroll
               for (int x = 0; x < 4; ++x)
-                if (x < x0 || x >= x0 + COLS / 32) tmem_st_32x16(s_addr + x * 16, none);
+                if (x < x0 || x >= x0 + COLS / 32) tmem_st_32x16(p_addr + x * 16, none);
             }
 #pragma unroll 1
             for (int x = x0; x < x0 + (COLS + 63) / 64 * 2; x += 2) {
@@ -585,6 +626,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                 tmem_ld_32x32(s_addr + 32 * x, ra);
                 tmem_ld_32x32(s_addr + 32 * x + 32, rb);
                 tmem_ld_wait();
+                release();
                 if (masked) {
                   hide(ra, x);
                   hide(rb, x + 1);
