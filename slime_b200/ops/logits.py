@@ -11,6 +11,7 @@ import torch
 from slime_b200.ops import _checks, _lib, reference, tree as _tree
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+MAX_VOCAB = 1 << 25  # the kernels sort tokens into 1024 buckets, each of which is within a table of 32768 tokens
 _CALL = struct.Struct("28q").pack  # arguments of the C entry
 
 
@@ -51,7 +52,7 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     S = R if cu_nodes is None else cu_nodes.shape[0] - 1
     penal = repetition is not None or frequency is not None or presence is not None
     # (as in ``tree.tree_attention``: one expression for what is in order)
-    fine = (out is None or (out.shape == logits.shape and out.dtype is dtype and out.device == dev and (V <= 1 or out.stride(1) == 1)))
+    fine = V <= MAX_VOCAB and (out is None or (out.shape == logits.shape and out.dtype is dtype and out.device == dev and (V <= 1 or out.stride(1) == 1)))
     if fine and penal:
         fine = (tokens is not None and lengths is not None and tokens.dim() == 2 and tokens.shape[0] == S and tokens.dtype is _I32 and tokens.device == dev
                 and (tokens.shape[1] <= 1 or tokens.stride(1) == 1) and lengths.shape == (S,) and lengths.dtype is _I32 and lengths.device == dev
@@ -102,6 +103,8 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
 def _check(logits, tokens, lengths, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, tree, out, S: int, penal: bool):
     """Raises on what ``adjust_logits`` does not take."""
     op, dev, (R, V) = "adjust_logits", logits.device, logits.shape
+    if V > MAX_VOCAB:
+        raise ValueError(f"{op}: a vocabulary of at most {MAX_VOCAB} tokens, not {V}")
     if tree is not None:
         drafted, parents, cu_nodes = tree
         _tree.check_trees(op, R, cu_nodes, _tree.MAX_NODES, drafted=drafted, parents=parents)

@@ -269,6 +269,91 @@ def test_logits_of_a_whole_vocabulary_in_a_graph():
     assert ops.adjust_logits(y[:0], allowed=torch.zeros(0, -(-V // 32), dtype=torch.int32, device="cuda")).shape == (0, V)
 
 
+# (rows times pieces of 2048 logits are more than the GPU holds at once: texts are counted by a kernel of their own)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("S, V, sizes, L, K", [(600, 4200, None, 70, 3), (40, 4099, [13, 0, 30, 75] * 10, 200, 5), (7, 6145, [128, 0, 90, 128, 1, 128, 128], 500, 300)])
+def test_logits_of_many_rows(dtype, S, V, sizes, L, K):
+    from slime_b200 import ops
+
+    x, kw, dev = logits_case(S, V, sizes, L=L, K=K, dtype=dtype)
+    want, _ = oracle.adjusted(x, **kw)
+    y = x.cuda()
+    a = ops.adjust_logits(y, **dev)
+    same_logits(a, want, dtype, spread=40 + K)
+    assert torch.equal(a.nan_to_num(9.0), ops.adjust_logits(y, **dev).nan_to_num(9.0))
+    assert torch.equal(y.nan_to_num(9.0).cpu(), x.nan_to_num(9.0))
+    assert ops.adjust_logits(y, **dev, out=y) is y
+    assert torch.equal(a.nan_to_num(9.0), y.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("parts", [(), ("repetition",), ("frequency",), ("presence",), ("bias",), ("allowed",), ("repetition", "allowed")])
+@pytest.mark.parametrize("sizes", [None, [2, 0, 100, 57] * 4])
+def test_logits_parts_alone_of_many_rows(parts, sizes):
+    from slime_b200 import ops
+
+    x, kw, dev = logits_case(640 if sizes is None else len(sizes), 4101, sizes, parts=parts)
+    want, _ = oracle.adjusted(x, **kw)
+    same_logits(ops.adjust_logits(x.cuda(), **dev), want, torch.float32)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("L", [6143, 6145, 12289, 40000])
+def test_logits_of_long_texts(dtype, L):
+    """Texts of every length up to L, tokens from the whole vocabulary and from a few; the same token all along; no text; a bias at either end, one of them twice."""
+    from slime_b200 import ops
+
+    S, V, sizes = 6, 20011, [40, 1, 0, 50, 24, 10]
+    x, kw, dev = logits_case(S, V, sizes, L=L, K=9, dtype=dtype)
+    g = torch.Generator().manual_seed(L)
+    kw["tokens"] = torch.randint(-1, V + 1, (S, L), generator=g, dtype=torch.int32)
+    kw["tokens"][1] %= 64
+    kw["tokens"][3] = 77
+    kw["tokens"][4, 1:] = V - 1
+    kw["lengths"] = torch.tensor([L, L - 1, 5, L, L // 2, 0], dtype=torch.int32)
+    kw["prompt_lens"] = torch.tensor([L // 3, 0, 5, L - 2, L, 0], dtype=torch.int32)
+    kw["bias_ids"][0, :3] = torch.tensor([V - 1, 0, V - 1])
+    dev = {n: tuple(t.cuda() for t in v) if isinstance(v, tuple) else v.cuda() for n, v in kw.items()}
+    want, _ = oracle.adjusted(x, **kw)
+    # (a frequency below one times up to L answers: one rounding of the product, one of the difference)
+    same_logits(ops.adjust_logits(x.cuda(), **dev), want, dtype, spread=40 + L)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_of_many_strided_rows_in_a_graph(dtype):
+    from slime_b200 import ops
+
+    sizes, V = [60, 128, 0, 128, 3, 100, 128], 4097
+    x, kw, dev = logits_case(7, V, sizes, dtype=dtype, L=90)
+    R = sum(sizes)
+    drafted, parents, cu = dev["tree"]
+    pad = lambda t: torch.cat([t, t[:2]])  # noqa: E731
+    dev["tree"], dev["allowed"] = (pad(drafted), pad(parents), cu), pad(dev["allowed"])
+    for left, right in ((1, 4), (0, 5), (3, 8)):
+        wide = torch.full((R + 2, left + V + right), 7.0, dtype=dtype, device="cuda")
+        wide[:, left : left + V] = pad(x.cuda())
+        out = torch.full((R + 2, V + 2 * left), 5.0, dtype=dtype, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.adjust_logits(wide[:, left : left + V], **dev, out=out[:, left : left + V])
+            ops.adjust_logits(wide[:, left : left + V], **dev, out=wide[:, left : left + V])
+        # the graph reads texts, lengths and trees as they are when it runs
+        cu_then = cu.clone()
+        for step in (0, 1):
+            if step:
+                wide[:, left : left + V] = pad(x.cuda())
+                out.fill_(5.0)
+                dev["tokens"].add_(3)
+                dev["lengths"].clamp_(max=60)
+            now = {**kw, "tokens": dev["tokens"].cpu(), "lengths": dev["lengths"].cpu()}
+            graph.replay()
+            want, _ = oracle.adjusted(x, **now)
+            for t in (out, wide):
+                same_logits(t[:R, left : left + V], want, dtype)
+            assert (out[R:] == 5).all() and (out[:, :left] == 5).all() and (out[:, left + V :] == 5).all()
+            assert (wide[:, :left] == 7).all() and (wide[:, left + V :] == 7).all()
+        assert torch.equal(cu, cu_then)
+
+
 # ------------------------------------------------------------------------------------------------------------- accept
 def accept_case(sizes, seed=0, share=0.8, holes=0.0):
     g = torch.Generator().manual_seed(seed)

@@ -1,5 +1,7 @@
 """Trees of drafted tokens, written node by node in 64 bits."""
 
+from collections import Counter
+
 import numpy as np
 import torch
 
@@ -93,9 +95,9 @@ def adjusted(logits, tokens=None, lengths=None, prompt_lens=None, repetition=Non
                 if 0 <= t < V:
                     f = num(repetition, b, 1.0)
                     x[r, t] = x[r, t] / f if x[r, t] > 0 else x[r, t] * f
-            for t in set(answer):
+            for t, times in Counter(answer).items():
                 if 0 <= t < V:
-                    x[r, t] -= num(frequency, b, 0.0) * answer.count(t) + num(presence, b, 0.0)
+                    x[r, t] -= num(frequency, b, 0.0) * times + num(presence, b, 0.0)
         if bias_ids is not None:
             for t, add in zip(bias_ids[b].tolist(), bias_values[b].tolist()):
                 if 0 <= t < V:
