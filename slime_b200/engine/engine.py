@@ -29,6 +29,7 @@ import numpy as np
 import torch
 
 from slime_b200 import ops
+from slime_b200.engine import penalties
 from slime_b200.engine.kv_cache import OutOfPages, PagedKVCache, _hash_block
 from slime_b200.engine.model_runner import EngineWeights, ModelRunner, cached_mixers
 from slime_b200.engine.request import ReqState, Request, SamplingParams
@@ -152,6 +153,7 @@ class Engine:
         self.h_pos = np.zeros(B, dtype=np.int64)  # position of the token the next step feeds
         self.h_remaining = np.zeros(B, dtype=np.int64)  # tokens still to sample (length limit)
         self.h_npages = np.zeros(B, dtype=np.int64)
+        self.h_adjusts = np.zeros(B, dtype=bool)  # the slot's logits are adjusted before they are sampled
         self.h_inspect = np.zeros(B, dtype=bool)  # slot needs its tokens looked at (EOS, stop ids, stop strings, stream)
         self.ring = int(min(max(self.max_context + 8, 64), 8192))
         pin = self.device.type == "cuda"
@@ -172,6 +174,7 @@ class Engine:
     # ------------------------------------------------------------------ intake
     def add_request(self, input_ids, sampling: SamplingParams | dict | None = None, rid: str | None = None, **kw) -> Request:
         sp = sampling if isinstance(sampling, SamplingParams) else SamplingParams.from_dict(sampling)
+        penalties.check(sp, rows=1 if self.spec is None else self.spec.k + 1)
         req = Request(rid=rid or uuid.uuid4().hex, input_ids=list(input_ids), sampling=sp, **kw)
         # Without an explicit seed the stream is numbered by arrival order: the ranks of a tensor-parallel engine see the
         # same requests in the same order, so they draw the same tokens (a hash of the random request id would differ
@@ -528,6 +531,7 @@ class Engine:
         if self.runner.recurrent:
             raise NotImplementedError("prefill / decode disaggregation does not carry the recurrent state of a request")
         sp = sampling if isinstance(sampling, SamplingParams) else SamplingParams.from_dict(sampling)
+        penalties.check(sp)
         req = Request(rid=rid or uuid.uuid4().hex, input_ids=list(input_ids), sampling=sp, **kw)
         self._req_counter = getattr(self, "_req_counter", 0) + 1
         req.seed = sp.sampling_seed if sp.sampling_seed is not None else (self.args.random_seed * 1000003 + self._req_counter) & 0x7FFFFFFFFFFF
@@ -572,6 +576,7 @@ class Engine:
         mp = f([r.sampling.min_p for r in reqs], torch.float32) if filtered else None
         seeds = f([r.seed for r in reqs], torch.int64)
         pos = f([len(r.output_ids) for r in reqs], torch.int32)
+        penalties.adjust(logits[:n], reqs)
         tok, lp, kept_ids, kept_cnt = ops.sample(logits[:n], temp, tk, tp, mp, seeds, pos, cap)
         self.stats["d2h_bytes"] += 8 * n
         return tok.tolist(), lp.tolist(), (kept_ids.cpu() if kept_ids is not None else None), (
@@ -601,6 +606,8 @@ class Engine:
         h["init_prev"][b], h["state_slot"][b] = (r.output_ids[-2] if len(r.output_ids) > 1 else r.input_ids[-1]), r.state_slot or 0
         h["top_k"][b], h["temperature"][b] = max(r.sampling.top_k, 0), r.sampling.temperature
         h["top_p"][b], h["min_p"][b], h["seeds"][b] = r.sampling.top_p, r.sampling.min_p, r.seed
+        self.runner.set_adjustments(b, r)
+        self.h_adjusts[b] = r.sampling.adjusts
         bt = h["block_table"][b]
         bt[:] = 0
         bt[: len(r.pages)] = r.pages
@@ -660,7 +667,7 @@ class Engine:
         filtered = bool((h["top_k"][:n][act[:n]] > 0).any() or (h["top_p"][:n][act[:n]] < 1.0).any() or (h["min_p"][:n][act[:n]] > 0).any())
         cap = 4096 if filtered and any(r.sampling.return_top_p_token_ids for r in self.running) else 0
         self.stats["h2d_bytes"] += self.runner.upload_static()
-        tok, lp, kept_ids, kept_cnt = self.runner.decode(n, filtered, cap)
+        tok, lp, kept_ids, kept_cnt = self.runner.decode(n, filtered, cap, bool((act & self.h_adjusts).any()))
         # results stream back into the pinned history ring; an event marks their arrival
         slot = self.step_no % self.ring
         self.tok_hist[slot, :n].copy_(tok[:n], non_blocking=True)

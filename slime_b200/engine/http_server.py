@@ -270,7 +270,8 @@ class EngineServer:
     def _openai_sampling(body: dict) -> dict:
         sp = {"max_new_tokens": int(body.get("max_tokens") or body.get("max_completion_tokens") or 128)}
         for src, dst in (("temperature", "temperature"), ("top_p", "top_p"), ("top_k", "top_k"), ("min_p", "min_p"),
-                         ("stop", "stop"), ("seed", "sampling_seed")):  # fmt: skip
+                         ("stop", "stop"), ("seed", "sampling_seed"), ("repetition_penalty", "repetition_penalty"),
+                         ("frequency_penalty", "frequency_penalty"), ("presence_penalty", "presence_penalty"), ("logit_bias", "logit_bias")):  # fmt: skip
             if body.get(src) is not None:
                 sp[dst] = body[src]
         return sp

@@ -17,7 +17,7 @@ import re
 import torch
 
 from slime_b200 import ops
-from slime_b200.engine import native_layer
+from slime_b200.engine import native_layer, penalties
 from slime_b200.engine.kv_cache import PagedKVCache
 from slime_b200.engine.projections import LayerProjections
 from slime_b200.engine.state_cache import RecurrentStates, StateShape
@@ -810,6 +810,7 @@ class ModelRunner:
             self.scale = mixers.mla_softmax_scale(cfg)
         self._native_layers = native_layer.covers(self)  # prefill of fresh prompts issues a layer at a time
         self.graphs: dict[int, tuple] = {}
+        self.adjustments = None  # of the decode slots, from the first request on that asks for any
         self.replayed_launches = 0  # kernel-library launches executed through graph replays
         self.graph_buckets = [b for b in (1, 2, 4, 8, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512) if b <= max_batch]
         if max_batch not in self.graph_buckets:
@@ -1431,8 +1432,19 @@ class ModelRunner:
         self.host["init_mask"][:] = 0
         return stage.numel() * 4
 
-    def _decode_step(self, n: int, filtered: bool, kept_cap: int):
-        """prepare -> model -> sample -> advance for slots [0, n). Returns (tokens, logprobs, kept_ids, kept_cnt, routed
+    def set_adjustments(self, slot: int, req):
+        """What the request that starts in ``slot`` asks of its logits (engine/penalties.py)."""
+        if self.adjustments is None:
+            if not req.sampling.adjusts:
+                return
+            self.adjustments = penalties.SlotAdjustments(self.max_batch, self.max_context, self.device)
+        if self.adjustments.set(slot, req):
+            if self.device.type == "cuda":
+                torch.cuda.current_stream().synchronize()
+            self.graphs = {k: g for k, g in self.graphs.items() if not k[3]}
+
+    def _decode_step(self, n: int, filtered: bool, kept_cap: int, adjust: bool = False):
+        """prepare -> model -> adjust -> sample -> advance for slots [0, n). Returns (tokens, logprobs, kept_ids, kept_cnt, routed
         experts, logits)."""
         w = self.w
         st, ds = self._static, self._dev_state
@@ -1451,6 +1463,8 @@ class ModelRunner:
             self._prepare_reference(n)
         h = self._decode_layers(n, ids, pos, slots, bt, seq_lens)
         logits = self.logits_of(h)
+        if adjust:
+            logits = self.adjustments.step(logits, ids, pos, seq_lens, st["active"][:n])
         tok, lp, kept_ids, kept_cnt = ops.sample(
             logits, st["temperature"][:n], st["top_k"][:n] if filtered else None, st["top_p"][:n] if filtered else None,
             st["min_p"][:n] if filtered else None, st["seeds"][:n], ds["out_pos"][:n], kept_cap,
@@ -1533,25 +1547,25 @@ class ModelRunner:
         ds["slots"][:n] = torch.where(act, slot, idle).to(torch.int32)
 
     @torch.no_grad()
-    def decode(self, n: int, filtered: bool, kept_cap: int = 0):
+    def decode(self, n: int, filtered: bool, kept_cap: int = 0, adjust: bool = False):
         """One decode step over slots [0, n) (host state must have been uploaded). Under CUDA graphs the
         step is one replay of the bucket that covers ``n``; extra slots are inactive by construction. MoE layers are
         captured too: their expert-sorted layout is built on the device with static shapes. ``last_routed`` holds the
         step's expert choices when ``record_routed`` is set (a buffer of the graph: copy it before the next replay)."""
         if not self.use_cuda_graph:
-            *outs, self.last_routed, self.last_logits = self._decode_step(n, filtered, kept_cap)
+            *outs, self.last_routed, self.last_logits = self._decode_step(n, filtered, kept_cap, adjust)
             return tuple(outs)
         bucket = next(b for b in self.graph_buckets if b >= n)
-        key = (bucket, filtered, kept_cap)
+        key = (bucket, filtered, kept_cap, adjust)
         if key not in self.graphs:
-            self._capture(bucket, filtered, kept_cap)
+            self._capture(*key)
         graph, outs, n_kernels = self.graphs[key]
         self.replayed_launches += n_kernels
         graph.replay()
         self.last_routed, self.last_logits = outs[4], outs[5]
         return outs[:4]
 
-    def _capture(self, bucket, filtered, kept_cap):
+    def _capture(self, bucket, filtered, kept_cap, adjust):
         """Capture one decode step. Warm-up and capture run with every slot inactive, so they only touch the
         reserved scratch page and leave the device-owned request state unchanged."""
         from slime_b200.ops import _lib
@@ -1564,13 +1578,13 @@ class ModelRunner:
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):
             for _ in range(2):
-                self._decode_step(bucket, filtered, kept_cap)
+                self._decode_step(bucket, filtered, kept_cap, adjust)
         torch.cuda.current_stream().wait_stream(side)
         g = torch.cuda.CUDAGraph()
         before = _lib.launch_count()
         with torch.cuda.graph(g):
-            outs = self._decode_step(bucket, filtered, kept_cap)
-        self.graphs[(bucket, filtered, kept_cap)] = (g, outs, _lib.launch_count() - before)
+            outs = self._decode_step(bucket, filtered, kept_cap, adjust)
+        self.graphs[(bucket, filtered, kept_cap, adjust)] = (g, outs, _lib.launch_count() - before)
         self._static["active"].copy_(saved_active)
         self._static["init_mask"].copy_(saved_init)
 

@@ -1,0 +1,111 @@
+"""What requests ask of their logits before a token is drawn: repetition, frequency and presence penalties and biases of tokens
+(``ops.adjust_logits``). Same fields as the ``sampling_params`` of the ``/generate`` payload that the reference's rollouts send
+(slime/rollout/sglang_rollout.py:152-221); returned log-probabilities are those of the adjusted distribution.
+
+Requests that ask for nothing pass through untouched, and a batch in which nobody asks launches nothing."""
+
+from __future__ import annotations
+
+import torch
+
+from slime_b200 import ops
+from slime_b200.ops import tree as tree_ops
+
+
+def check(sampling, rows: int = 1):
+    """Raises ValueError on penalties that have no meaning, and where a pass has more ``rows`` for a request than a tree of the operator has nodes."""
+    if sampling.adjusts and rows > tree_ops.MAX_NODES:
+        raise ValueError(f"penalties take chains of at most {tree_ops.MAX_NODES - 1} guesses, not {rows - 1}")
+    if not sampling.repetition_penalty > 0:
+        raise ValueError(f"repetition_penalty must be above zero, not {sampling.repetition_penalty}")
+
+
+def adjust(logits, reqs, chains=None):
+    """Logits of ``reqs`` adjusted in place, a row for each; nothing happens if no request asks. ``chains`` = (ids, cu): request b has the rows cu[b] .. cu[b + 1]
+    for the last token of its text and the guesses behind it, which the device tensors ``ids`` and ``cu`` name."""
+    if not any(r.sampling.adjusts for r in reqs):
+        return logits
+    dev, B = logits.device, len(reqs)
+    texts = [r.all_ids() if r.sampling.adjusts else [] for r in reqs]
+    lens = torch.tensor([len(t) for t in texts], dtype=torch.int32)
+    tokens = torch.zeros(B, max(int(lens.max()), 1), dtype=torch.int32)
+    for row, text in zip(tokens, texts):
+        row[: len(text)] = torch.tensor(text, dtype=torch.int32)
+    numbers = torch.tensor([_numbers(r.sampling) for r in reqs], dtype=torch.float32).t().contiguous().to(dev)
+    ids, values = _biases([r.sampling for r in reqs])
+    tree = None
+    if chains is not None:
+        drafted, cu = chains
+        at = torch.arange(drafted.shape[0], device=dev, dtype=torch.int32)
+        owner = torch.searchsorted(cu, at, right=True) - 1
+        tree = (drafted, at - cu[owner] - 1, cu)  # a guess hangs on the one before it, the first row on nothing (-1)
+    return ops.adjust_logits(
+        logits, tokens.to(dev), lens.to(dev), torch.tensor([len(r.input_ids) for r in reqs], dtype=torch.int32).to(dev), repetition=numbers[0],
+        frequency=numbers[1], presence=numbers[2], bias_ids=None if ids is None else ids.to(dev), bias_values=None if ids is None else values.to(dev),
+        tree=tree, out=logits)  # fmt: skip
+
+
+def _numbers(s):
+    return s.repetition_penalty, s.frequency_penalty, s.presence_penalty
+
+
+def _biases(samplings):
+    """([B, K] token ids, -1 behind the last; [B, K] values), or (None, None)."""
+    K = max(len(s.logit_bias or ()) for s in samplings)
+    if K == 0:
+        return None, None
+    ids, values = torch.full((len(samplings), K), -1, dtype=torch.int32), torch.zeros(len(samplings), K)
+    for b, s in enumerate(samplings):
+        if s.logit_bias:
+            n = len(s.logit_bias)
+            ids[b, :n] = torch.tensor(list(s.logit_bias), dtype=torch.int32)
+            values[b, :n] = torch.tensor(list(s.logit_bias.values()), dtype=torch.float32)
+    return ids, values
+
+
+class SlotAdjustments:
+    """The same for decode slots, whose texts the host does not know up to the last token: the device keeps them, a step adds the token that it is fed."""
+
+    def __init__(self, slots: int, max_context: int, device):
+        self.text = torch.zeros(slots, max_context + 1, dtype=torch.int32, device=device)
+        self.prompt_lens = torch.zeros(slots, dtype=torch.int32, device=device)
+        self.numbers = torch.zeros(3, slots, device=device)
+        self.numbers[0] = 1.0
+        self.bias_ids = self.bias_values = None
+        self.asked = [False] * slots
+
+    def set(self, slot: int, req) -> bool:
+        """The slot's next steps are of this request. True: the buffers of the biases are others now, and a captured step is stale."""
+        s = req.sampling
+        if not (s.adjusts or self.asked[slot]):
+            return False
+        self.asked[slot] = s.adjusts
+        dev = self.text.device
+        self.numbers[:, slot] = torch.tensor(_numbers(s), dtype=torch.float32).to(dev)
+        if s.adjusts:
+            ids = torch.tensor(req.all_ids(), dtype=torch.int32)
+            self.text[slot, : len(ids)] = ids.to(dev)
+            self.prompt_lens[slot] = len(req.input_ids)
+        ids, values = _biases([s])
+        need, have = 0 if ids is None else ids.shape[1], 0 if self.bias_ids is None else self.bias_ids.shape[1]
+        if need > have:
+            room = max(16, 1 << (need - 1).bit_length())
+            grown = (torch.full((self.text.shape[0], room), -1, dtype=torch.int32, device=dev), torch.zeros(self.text.shape[0], room, device=dev))
+            if have:
+                grown[0][:, :have], grown[1][:, :have] = self.bias_ids, self.bias_values
+            self.bias_ids, self.bias_values = grown
+        if self.bias_ids is not None:
+            self.bias_ids[slot] = -1
+            if need:
+                self.bias_ids[slot, :need], self.bias_values[slot, :need] = ids[0].to(dev), values[0].to(dev)
+        return need > have
+
+    def step(self, logits, ids, pos, seq_lens, active):
+        """Logits of the first slots adjusted in place. The token that a slot was fed, ``ids`` at ``pos``, joins its text; idle slots keep theirs."""
+        n = logits.shape[0]
+        text, at = self.text[:n], pos.long()[:, None]
+        text.scatter_(1, at, torch.where(active[:, None] != 0, ids[:, None], text.gather(1, at)))
+        some = self.bias_ids is not None
+        return ops.adjust_logits(
+            logits, text, seq_lens, self.prompt_lens[:n], repetition=self.numbers[0, :n], frequency=self.numbers[1, :n], presence=self.numbers[2, :n],
+            bias_ids=self.bias_ids[:n] if some else None, bias_values=self.bias_values[:n] if some else None, out=logits)  # fmt: skip

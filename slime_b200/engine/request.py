@@ -25,7 +25,10 @@ class SamplingParams:
     no_stop_trim: bool = False
     spaces_between_special_tokens: bool = True
     sampling_seed: int | None = None
-    repetition_penalty: float = 1.0
+    repetition_penalty: float = 1.0  # a logit above zero of a token of prompt or answer is divided by it, any other multiplied
+    frequency_penalty: float = 0.0  # subtracted once for each time that the answer has the token ...
+    presence_penalty: float = 0.0  # ... and once if it has it
+    logit_bias: dict[int, float] | None = None  # added to the logits of these tokens
     n: int = 1
     custom_params: dict[str, Any] | None = None
 
@@ -38,7 +41,15 @@ class SamplingParams:
             sp.stop = [sp.stop]
         if sp.top_k is None or sp.top_k <= 0:
             sp.top_k = -1
+        for name, neutral in (("repetition_penalty", 1.0), ("frequency_penalty", 0.0), ("presence_penalty", 0.0)):
+            setattr(sp, name, neutral if getattr(sp, name) is None else float(getattr(sp, name)))
+        sp.logit_bias = {int(t): float(v) for t, v in sp.logit_bias.items()} if sp.logit_bias else None  # (JSON's keys are texts)
         return sp
+
+    @property
+    def adjusts(self) -> bool:
+        """Whether logits are changed before they are sampled."""
+        return self.repetition_penalty != 1.0 or self.frequency_penalty != 0.0 or self.presence_penalty != 0.0 or bool(self.logit_bias)
 
     @property
     def return_top_p_token_ids(self) -> bool:

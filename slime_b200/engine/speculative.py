@@ -32,6 +32,7 @@ import time
 import torch
 
 from slime_b200 import ops
+from slime_b200.engine import penalties
 from slime_b200.engine.kv_cache import OutOfPages
 from slime_b200.engine.request import Request
 
@@ -150,6 +151,8 @@ class SpeculativeDecoder:
         sp = [r.sampling for r in row_req]
         filtered = any(s.top_k > 0 or s.top_p < 1.0 or s.min_p > 0 for s in sp)
         cap = 4096 if filtered and any(s.return_top_p_token_ids for s in sp) else 0
+        if any(r.sampling.adjusts for r, _, _ in spans):
+            logits = penalties.adjust(logits, [r for r, _, _ in spans], (eng._to_dev(ids), cu))
         tok, lp, kept_ids, kept_cnt = ops.sample(
             logits, f([s.temperature for s in sp], torch.float32), f([max(s.top_k, 0) for s in sp], torch.int32) if filtered else None,
             f([s.top_p for s in sp], torch.float32) if filtered else None, f([s.min_p for s in sp], torch.float32) if filtered else None,

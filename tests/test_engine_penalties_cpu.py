@@ -1,0 +1,82 @@
+"""Penalties and biases of requests in the engine: every token is the best (or the drawn one) of its adjusted logits, with slots, retraction and chains of guesses."""
+
+import numpy as np
+import pytest
+import torch
+import tree_oracle
+from test_engine_cpu import make_engine
+from test_engine_speculative_cpu import _pair, _prompts
+
+from slime_b200.engine.http_server import EngineServer
+from slime_b200.engine.request import SamplingParams
+
+ASKS = [dict(repetition_penalty=1.7), dict(frequency_penalty=0.6, presence_penalty=0.3), dict(), dict(logit_bias={"5": 2.5, 7: -100.0, 10**6: 3.0}),
+        dict(repetition_penalty=0.8, frequency_penalty=-0.2, presence_penalty=0.5, logit_bias={3: 0.5})]  # fmt: skip
+
+
+@pytest.mark.parametrize("greedy", [True, False])
+def test_slots_draw_from_adjusted_logits(greedy):
+    _, _, plain, spec = _pair("dense")
+    cfg = plain.cfg
+    prompts = _prompts(cfg, len(ASKS))
+    sampling = dict(max_new_tokens=20, ignore_eos=True, **(dict(temperature=0) if greedy else dict(temperature=1.0, sampling_seed=9)))
+    reqs = plain.generate(prompts, [dict(sampling, **a) for a in ASKS])
+    # a step's tokens from single prefills of everything in front of them, whose logits are adjusted by the oracle
+    for r, a in zip(reqs, ASKS):
+        n, s = len(r.input_ids), r.sampling
+        bias = {int(t): v for t, v in (a.get("logit_bias") or {}).items()}
+        for i in (0, 1, 7, 19):
+            ids = r.input_ids + r.output_ids[:i]
+            seen = {}
+
+            def keep(logits, reqs, chains=None, seen=seen):
+                seen["x"] = logits.clone()
+                return logits
+
+            with pytest.MonkeyPatch.context() as m:
+                m.setattr("slime_b200.engine.penalties.adjust", keep)
+                plain.generate([ids], dict(max_new_tokens=1, ignore_eos=True))
+            f = lambda x: torch.tensor([x])  # noqa: E731
+            x, _ = tree_oracle.adjusted(seen["x"], torch.tensor([ids]), torch.tensor([len(ids)]), torch.tensor([n]), f(s.repetition_penalty),
+                                        f(s.frequency_penalty), f(s.presence_penalty), torch.tensor([list(bias)], dtype=torch.int32) if bias else None,
+                                        torch.tensor([list(bias.values())]) if bias else None)  # fmt: skip
+            lp = torch.log_softmax(x[0], -1)
+            assert abs(float(lp[r.output_ids[i]]) - r.output_logprobs[i]) < 2e-4
+            if greedy:
+                assert r.output_ids[i] == int(lp.argmax())
+    # the request that asks for nothing is the one that it is alone, and what a slot was asked is forgotten with its request
+    assert plain.generate([prompts[2]], dict(sampling))[0].output_ids == reqs[2].output_ids
+    # chains of guesses
+    for x, y in zip(reqs, spec.generate(prompts, [dict(sampling, **a) for a in ASKS])):
+        assert x.output_ids == y.output_ids
+        assert np.abs(np.array(x.output_logprobs) - np.array(y.output_logprobs)).max() < 2e-4
+
+
+def test_a_request_that_is_put_back_keeps_its_penalties():
+    ask = dict(max_new_tokens=24, ignore_eos=True, frequency_penalty=0.7, presence_penalty=0.2, repetition_penalty=1.2)
+    prompts = [[i + 1] * 6 for i in range(4)]
+    small, big = make_engine(pages=14, max_running=4), make_engine(pages=200, max_running=4)
+    a, b = (e.generate(prompts, [dict(ask, sampling_seed=i) for i in range(4)]) for e in (small, big))
+    assert [r.output_ids for r in a] == [r.output_ids for r in b]
+    never = big.generate([prompts[0]], dict(max_new_tokens=30, ignore_eos=True, temperature=0, presence_penalty=1e4))[0]
+    assert len(set(never.output_ids)) == 30  # no token twice
+
+
+def test_biases_of_more_tokens_than_any_request_before():
+    _, _, plain, _ = _pair("dense")
+    prompt = _prompts(plain.cfg, 1)[0]
+    for allowed in ([4], list(range(30)), [4]):
+        bias = {t: -1e9 for t in range(plain.cfg.vocab_size) if t not in allowed}
+        got = plain.generate([prompt, prompt], [dict(max_new_tokens=6, ignore_eos=True, logit_bias=bias), dict(max_new_tokens=6, ignore_eos=True)])
+        assert set(got[0].output_ids) <= set(allowed)
+
+
+def test_penalties_as_they_arrive():
+    sp = SamplingParams.from_dict(dict(repetition_penalty=None, frequency_penalty=None, presence_penalty=None, logit_bias=None))
+    assert not sp.adjusts and sp == SamplingParams()
+    assert SamplingParams.from_dict(dict(logit_bias={"12": -3})).logit_bias == {12: -3.0}
+    assert EngineServer._openai_sampling(dict(frequency_penalty=0.5, presence_penalty=1, logit_bias={"3": 1}))["frequency_penalty"] == 0.5
+    _, _, plain, _ = _pair("dense")
+    for bad in (0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="repetition_penalty"):
+            plain.add_request([1, 2], dict(repetition_penalty=bad))

@@ -494,3 +494,32 @@ def test_a_round_of_drafted_trees_is_ordinary_decoding():
     for b in range(B):
         at = torch.tensor([oracle.slot(table, b, p, page) for p in range(ctx[b])], device="cuda")
         assert torch.equal(k2[0, at], k1[0, at]) and torch.equal(v2[0, at], v1[0, at])
+
+
+# ------------------------------------------------------------------------------------------------------- in the engine
+def test_captured_decode_steps_adjust_their_logits():
+    """Requests with penalties and biases beside one without: eager and replayed steps draw the same tokens, a later request in a
+    used slot is what it is alone, and biases of more tokens than any request had before are taken up."""
+    from slime_b200.engine.engine import Engine
+    from slime_b200.engine.server_args import ServerArgs
+    from slime_b200.models.config import get_preset
+
+    prompts = [[(5 * i + 3 * j) % 500 for j in range(6 + i)] for i in range(4)]
+    many = {t: -1e9 for t in range(100, 500)}
+    asks = [dict(repetition_penalty=1.3), dict(frequency_penalty=0.4, presence_penalty=0.2), dict(), dict(logit_bias={7: 3.0, 9: -100.0}, repetition_penalty=0.9)]
+    got = []
+    for graphs in (False, True):
+        e = Engine(get_preset("tiny"), ServerArgs(page_size=16, max_running_requests=4, context_length=128, disable_cuda_graph=not graphs),
+                   device="cuda", num_pages=64)  # fmt: skip
+        e.weights.init_random(0, std=0.2)
+        base = dict(max_new_tokens=20, temperature=0, ignore_eos=True)
+        first = e.generate(prompts, [dict(base, **a) for a in asks])
+        assert bool(e.runner.graphs) == graphs
+        plain = e.generate(prompts, dict(base))
+        assert first[2].output_ids == plain[2].output_ids and 9 not in first[3].output_ids
+        again = e.generate(prompts, [dict(base, logit_bias=many if i == 1 else None, presence_penalty=1e4 if i == 0 else 0) for i in range(4)])
+        assert len(set(again[0].output_ids)) == 20 and not set(again[1].output_ids) & set(many)
+        assert [r.output_ids for r in again[2:]] == [r.output_ids for r in plain[2:]]
+        got.append([[r.output_ids for r in x] + [r.output_logprobs for r in x] for x in (first, plain, again)])
+        e.shutdown()
+    assert got[0] == got[1]
