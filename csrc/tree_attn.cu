@@ -65,9 +65,9 @@ tree_attn_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const T
       for (int d = 0; d < D; ++d) s = fmaf(q_s[warp][d], static_cast<float>(row[d]), s);
       s *= c;
     }
-    const float top = fmaxf(m, warp_max(s));
-    if (top == -INFINITY) continue;
-    const float keep = exp2f(m - top), p = exp2f(s - top);
+    if (!__any_sync(0xffffffffu, sees)) continue;
+    const float top = fmaxf(m, warp_max(s)), zero = top == -INFINITY ? 0.f : top;  // (maxima leave NaN out, the weights below do not)
+    const float keep = exp2f(m - zero), p = exp2f(s - zero);
     m = top;
     l = l * keep + p;
 #pragma unroll
@@ -84,7 +84,7 @@ tree_attn_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const T
   }
   l = warp_sum(l);
   if (sinks != nullptr && m != -INFINITY) l += exp2f(sinks[h] * 1.4426950408889634f - m);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
   for (int x = 0; x < TA_MAXD / 32; ++x)
     if (x * 32 + lane < D) out[t * out_row + static_cast<long>(h) * D + x * 32 + lane] = static_cast<T>(acc[x] * inv);

@@ -27,7 +27,8 @@
 // waiter sees every phase of a barrier: a wait by parity cannot tell one phase from the next but one. Even rings give that to the groups, which
 // take tiles in turn; a ring of three buffers has six barriers for it. The scores of hidden nodes become -infinity by a bit mask per row, looked at in the last tiles only. Cache rows behind
 // the last node may hold anything: pages behind it are fetched from outside the cache, which reads as zero, and the rest of its page is
-// cleared in shared memory before the product of weights (zero) and values.
+// cleared in shared memory before the product of weights (zero) and values. So are nodes' values that are not finite: rows that see
+// such a node become NaN, and the others stay what they are.
 // Every wait is bounded: on expiry the CTA records a status word, drains and returns with its TMEM freed.
 #include <type_traits>
 
@@ -66,6 +67,28 @@ __device__ __noinline__ bool tt_wait_long(uint64_t* bar, uint32_t parity, volati
 }
 __device__ __forceinline__ bool tt_wait(uint64_t* bar, uint32_t parity, volatile int* cta_abort, int* status, int code) {
   return mbar_try_wait(bar, parity) || tt_wait_long(bar, parity, cta_abort, status, code);
+}
+// A group's 128 threads make values of hidden keys harmless (0 x NaN would reach O): rows [end, to) of a tile, behind the last key, are cleared, and
+// of rows [from, end), which are nodes from first_node on, 16-byte pieces that are not all finite; bad: such nodes.
+template <int NCH>
+__device__ __forceinline__ void tt_clean(uint8_t* v, int from, int end, int to, int first_node, int tid, uint32_t* bad) {
+#pragma unroll 1
+  for (int x = tid; x < (to - from) * (NCH * 8); x += 128) {
+    const int vr = from + x / (NCH * 8), ch = (x / 8) % NCH;
+    uint4* at = reinterpret_cast<uint4*>(v + ch * (TT_BN * 128) + vr * 128 + (x & 7) * 16);
+    bool clear = vr >= end;
+    if (!clear) {
+      const uint4 e = *at;
+      auto inf = [](uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; };
+      clear = inf(e.x) || inf(e.y) || inf(e.z) || inf(e.w);
+      if (clear) {
+        const int node = first_node + vr - from;
+        atomicOr(&bad[node >> 5], 1u << (node & 31));
+        __threadfence_block();  // before the other group can read zeros: it uses the tile too where a tree has two query tiles
+      }
+    }
+    if (clear) *at = make_uint4(0, 0, 0, 0);
+  }
 }
 __device__ __forceinline__ void tt_barrier(int id, int nthreads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory"); }
 
@@ -178,6 +201,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   volatile int* cta_abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* start = reinterpret_cast<int*>(tmem_slot + 2);  // [0] request, [1] unit within it
   int* sums = start + 2;                               // [12] units of the warps' requests
+  uint32_t* bad = reinterpret_cast<uint32_t*>(sums + 12);  // [2 pieces][4] nodes with values that are not finite
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int* status = a.status;
@@ -320,6 +344,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
           if (!ok) break;
           if (hides) {
+            if (lane < 4) bad[buf * 4 + lane] = 0;
             __syncwarp();
             for (int i = lane; i < walk.r.n; i += 32) {
               uint32_t set[4];
@@ -639,17 +664,12 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             f2_unpack(f2_add(sum[0], sum[1]), s0, s1);
             l_run += s0 + s1;
           }
-          if (ends && j + 1 == nt && (walk.keys & (page - 1)) != 0) {
-            // value rows behind the last key: the rest of its page is cleared (0 x NaN would reach O), by each group that uses the tile
+          if (masked) {  // values of nodes, and behind the last key: by each group that uses the tile
             const uint32_t t = t0 + j, vs = S::K_RING + t % S::V_RING;
             ok = __all_sync(0xffffffffu, tt_wait(&full[S::K_RING + t % S::V_FULL], t / S::V_FULL & 1, cta_abort, status, ERR_WAIT_FULL));
             if (!ok) break;
-            const int from = walk.keys & (TT_BN - 1), to = (from + page - 1) & -page;
-            uint8_t* v = sKV + vs * S::KV_TILE;
-            for (int x = tid; x < (to - from) * NCH * 8; x += 128) {
-              const int vr = from + x / (NCH * 8), ch = (x / 8) % NCH;
-              *reinterpret_cast<uint4*>(v + ch * (TT_BN * 128) + vr * 128 + (x & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
+            const int from = max(ctx - key0, 0), end = min(walk.keys - key0, TT_BN);
+            tt_clean<NCH>(sKV + vs * S::KV_TILE, from, end, (end + page - 1) & -page, key0 + from - ctx, tid, bad + (piece & 1) * 4);
             fence_proxy_async();
           }
           tmem_st_wait();
@@ -658,13 +678,11 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
           if (lane == 0) mbar_arrive(&p_full[g]);
         }
         s_cnt += n_my;
-        bool hole = false;
+        bool hole = false, poisoned = false;
         if ((walk.tile0 + nt) * TT_BN > ctx) {
           want_ways();
           hole = valid && (way[0] & 1) == 0;
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&w_empty[piece & 1]);
         // ---- epilogue: with one query tile the groups (and copies) are joined, and each group writes half of the columns
         const bool all = walk.tile0 == 0 && ends;
         const int slot = 2 * c + (piece == 0 ? 0 : 1);
@@ -696,15 +714,22 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         o_cnt0 += has0;
         o_cnt1 += has1;
         tc_fence_after();
+        if (valid && (walk.tile0 + nt) * TT_BN > ctx) {  // (every thread that looks at values of this piece's nodes has done so)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) poisoned |= (way[x] & bad[(piece & 1) * 4 + x]) != 0;
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w_empty[piece & 1]);
         float inv = 1.f;
         if (all) {
           const int head = walk.kvh * a.G + head_in;
           if (a.sinks != nullptr && valid && l > 0.f) l += tt_exp2(a.sinks[head] * 1.4426950408889634f - m);
-          inv = (l > 0.f && !hole) ? 1.f / l : 0.f;
+          inv = hole || l == 0.f ? 0.f : 1.f / l;  // (a sum that is NaN comes through)
         }
+        if (poisoned) inv = __int_as_float(0x7fffffff);
         // an accumulator that nothing was added to holds anything, and a row that sees nothing is zero whatever its accumulators hold
         const float by0 = f0 * inv, by1 = f1 * inv;
-        const uint32_t keep0 = has0 && by0 > 0.f ? 0xffffffffu : 0u, keep1 = has1 && by1 > 0.f ? 0xffffffffu : 0u;
+        const uint32_t keep0 = has0 && by0 != 0.f ? 0xffffffffu : 0u, keep1 = has1 && by1 != 0.f ? 0xffffffffu : 0u;
         auto both = [&](uint32_t x, uint32_t y) { return fmaf(__uint_as_float(x & keep0), by0, __uint_as_float(y & keep1) * by1); };
         if constexpr (REP == 1) {
           if (ok && active) {
@@ -722,7 +747,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               float v[16];
               if (rows2) {
 #pragma unroll
-                for (int k = 0; k < 16; ++k) v[k] = inv > 0.f ? __uint_as_float(x[k]) * inv : 0.f;
+                for (int k = 0; k < 16; ++k) v[k] = inv != 0.f ? __uint_as_float(x[k]) * inv : 0.f;
               } else {
 #pragma unroll
                 for (int k = 0; k < 16; ++k) v[k] = both(x[k], y[k]);
@@ -779,9 +804,9 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             tt_barrier(1 + g, 128);
           }
         }
-        // a node of no tree marks its row with an infinite maximum
+        // a node of no tree marks its row with a negative sum
         if (!all && valid && copy == 0 && (rows2 || g == 0))
-          a.part_ml[static_cast<long>(slot) * (128 * TILES) + qt * 128 + rr] = make_float2(hole ? INFINITY : m, l);
+          a.part_ml[static_cast<long>(slot) * (128 * TILES) + qt * 128 + rr] = make_float2(m, hole ? -1.f : l);
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(o_empty);
@@ -821,6 +846,7 @@ tree_attn_join_kernel(const __grid_constant__ TtArgs a) {
   // part p: in slot plan.y, or the first slot of the CTA behind
   auto at = [&](int p) { return static_cast<long>(p == 0 ? plan.y : 2 * (c + p)) * (128 * TILES) + x; };
   float top = -INFINITY, l = 0.f, o[V];
+  bool hole = false;
 #pragma unroll
   for (int i = 0; i < V; ++i) o[i] = 0.f;
   for (int p0 = 0; p0 < parts; p0 += 32) {
@@ -832,7 +858,8 @@ tree_attn_join_kernel(const __grid_constant__ TtArgs a) {
 #pragma unroll
       for (int i = 0; i < FLY; ++i)
         if (p1 + i < count) v[i] = *reinterpret_cast<const Vec*>(a.part_o + at(p0 + p1 + i) * D + lane * V);
-      if (p1 == 0) {  // what was added up so far, and these parts, on the scale of the largest maximum (infinite: the node of no tree)
+      if (p1 == 0) {  // what was added up so far, and these parts, on the scale of the largest maximum
+        hole = hole || __any_sync(0xffffffffu, mine.y < 0.f);
         new_top = fmaxf(top, warp_max(mine.x));
         const float keep = top == -INFINITY ? 0.f : tt_exp2(top - new_top);
         f = mine.x == -INFINITY ? 0.f : tt_exp2(mine.x - new_top);
@@ -854,7 +881,7 @@ tree_attn_join_kernel(const __grid_constant__ TtArgs a) {
   }
   const int head = plan.z * a.G + row - in_tile * a.G;
   if (a.sinks != nullptr) l += tt_exp2(a.sinks[head] * 1.4426950408889634f - top);
-  const bool some = top != INFINITY && top != -INFINITY && l > 0.f;
+  const bool some = !hole && l != 0.f;  // (a sum that is NaN comes through)
   const float inv = some ? 1.f / l : 0.f;
 #pragma unroll
   for (int k = 0; k < V; ++k) o[k] = some ? o[k] * inv : 0.f;

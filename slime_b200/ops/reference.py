@@ -185,12 +185,14 @@ def tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, par
                 sees[i, [ctx + j for j in ways[lo + i]]] = True
         ks = k_cache[slots].float().repeat_interleave(Hq // Hkv, dim=1)
         vs = v_cache[slots].float().repeat_interleave(Hq // Hkv, dim=1)
-        vs = torch.where(sees.any(0)[:, None, None], vs, 0.0)
+        bad = ~torch.isfinite(vs)  # a value that is not finite reaches the rows that see it, and no other
+        vs = torch.where(bad, 0.0, vs)
         x = torch.einsum("ihd,jhd->hij", q[lo:hi].float() * scale, ks).masked_fill(~sees, float("-inf"))
         if sinks is not None:
             x = torch.cat([x, sinks.float()[:, None, None].expand(Hq, hi - lo, 1)], dim=-1)
         p = torch.where(sees.any(1)[:, None], x.softmax(-1)[..., : sees.shape[1]], 0.0)
-        out[lo:hi] = torch.einsum("hij,jhd->ihd", p, vs).to(q.dtype)
+        got = torch.einsum("hij,jhd->ihd", p, vs)
+        out[lo:hi] = torch.where(torch.einsum("ij,jhd->ihd", sees.float(), bad.float()) > 0, math.nan, got).to(q.dtype)
     return out
 
 

@@ -123,8 +123,9 @@ def tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, par
     the nodes above it and itself; a node that belongs to no tree gets zeros. ``sinks`` [Hq] fp32: score of an extra softmax column without
     a value. ``max_nodes``: no tree has more nodes. Rows of ``out`` behind ``cu_nodes[B]`` are left as they are (a new ``out``: undefined).
 
-    Keys and values of hidden rows have weight zero and have to be finite where they belong to a tree; what stands in a page behind the
-    last node may be anything. bf16, and fp32 throughout; heads up to 256 wide."""
+    What a row does not see may be anything, NaN too: other branches, nodes of no tree, the rest of a page. A row that sees a value that
+    is not finite has no finite output (of a node: its head is NaN as a whole). bf16, and fp32 throughout; heads up to 256 wide. In batch-invariant mode a row's
+    bits depend on its own tree and ``max_nodes``, not on the requests beside it."""
     kv, dev, dtype, B = k_cache.shape, q.device, q.dtype, context_lens.shape[0]
     # (one expression for calls that are in order, which is most of what a call costs on the host; the check proper says what is wrong with others)
     if not (q.dim() == 3 and len(kv) == 3 and v_cache.shape == kv and kv[2] == q.shape[2] <= 256 and kv[1] > 0 and q.shape[1] % kv[1] == 0 and page_size > 0
@@ -184,7 +185,7 @@ def _check_caches(op: str, caches, block_table, context_lens, page_size, B: int,
     _shape(op, "block_table", block_table, B, None)
     _shape(op, "context_lens", context_lens, B)
     _ints(op, device, block_table=block_table, context_lens=context_lens)
-    groups = {}
+    groups, starts = {}, set()
     for c in caches:
         if c.device != device:
             raise ValueError(f"{op}: caches and trees are on one device")
@@ -194,6 +195,9 @@ def _check_caches(op: str, caches, block_table, context_lens, page_size, B: int,
         layers, step = (shape[0], strides[0] * n) if len(shape) == 4 else (1, 0)
         width = shape[-1] * shape[-2] * n
         if width and layers:  # (a cache of latents has no values)
+            if c.data_ptr() in starts:
+                raise ValueError(f"{op}: two caches share memory (values that are a view of the keys move with them)")
+            starts.add(c.data_ptr())
             groups.setdefault((layers, step, shape[-3], width, strides[-3] * n), []).append(c.data_ptr())
     return groups
 
@@ -207,6 +211,8 @@ def _two_stacks(k, v, block_table, context_lens, page_size, B: int, device):
             and strides[3] == 1 and strides[2] == shape[3] and shape[0] and page_size > 0 and block_table.dtype is _I32 and context_lens.dtype is _I32
             and block_table.device == device and context_lens.device == device and block_table.dim() == 2 and block_table.shape[0] == B
             and context_lens.shape == (B,) and block_table.is_contiguous() and context_lens.is_contiguous()):  # fmt: skip
+        return None
+    if k.data_ptr() == v.data_ptr():
         return None
     n = k.itemsize
     width = shape[2] * shape[3] * n
@@ -223,7 +229,8 @@ def accept_tree(sampled, drafted, parents, cu_nodes, max_nodes: int, *, k_caches
 
     With caches (a stacked tensor [layers, slots, heads, width] or a sequence of [slots, heads, width] each) the keys and values of the nodes on
     the path move, in place, to positions ``context_lens[b] + 0, 1, 2, ...``, so that the cache holds the accepted tokens in order. No page
-    that holds nodes of one request may belong to another."""
+    that holds nodes of one request may belong to another, and no two caches share memory (values that are a
+    view of the keys move with them and are left out)."""
     op, dev, rows = "accept_tree", cu_nodes.device, sampled.shape
     if not (0 < max_nodes <= MAX_NODES and len(rows) == 1 and cu_nodes.dim() == 1 and cu_nodes.shape[0] > 0 and drafted.shape == rows and parents.shape == rows
             and cu_nodes.dtype is _I32 and sampled.dtype is _I32 and drafted.dtype is _I32 and parents.dtype is _I32 and sampled.device == dev

@@ -105,6 +105,32 @@ def test_attention_strides_sinks_factors_and_pages(page, heads):
         assert (out[n:] == 7).all()
 
 
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 8, 128), (16, 1, 128), (8, 1, 128), (2, 2, 64), (4, 2, 8)])
+@pytest.mark.parametrize("sizes, ctx", [([8, 1], [120, 16]), ([31, 61, 2], [97, 3, 255]), ([128, 100, 9], [40, 300, 2000])])
+@pytest.mark.parametrize("what", ["keys", "values", "one value"])
+def test_attention_beside_numbers_that_are_not_finite(heads, sizes, ctx, what):
+    """NaN in nodes of no tree and in one node of each tree, infinities in a cached token of the last request: rows that see none of them are as ever, the others not finite."""
+    from slime_b200 import ops
+
+    page = 16
+    q, k, v, table, c, cu, parents = attention_case(sizes, ctx, heads, page, seed=3, holes=0.15)
+    par, starts = parents.tolist(), cu.tolist()
+    x = k if what == "keys" else v
+    last = slice(0, 1) if what == "one value" else slice(None)
+    for b, n in enumerate(sizes):
+        for i in range(n):
+            if i == n // 2 or (i > 0 and not oracle.way_up(par[starts[b] : starts[b + 1]], i)):
+                x[oracle.slot(table, b, ctx[b] + i, page), :, last] = math.nan
+    if len(sizes) > 2:
+        x[oracle.slot(table, 2, ctx[2] // 3, page), :, last] = math.inf
+    got = ops.tree_attention(q, k, v, table, c, cu, parents, page, max(sizes)).double().cpu()
+    want, mass = oracle.attention(q, k, v, table, c, cu, parents, page, heads[2] ** -0.5)
+    fine = want.isfinite()
+    assert not got[~fine].isfinite().any() and (~fine).any()
+    rows = fine.all(2) & mass.isfinite().all(2)
+    assert rows.any() and ((got - want).abs() <= bound(want, mass, torch.bfloat16, heads[2]))[rows].all()
+
+
 @pytest.mark.parametrize("shape", ["chain", "star"])
 def test_attention_of_chains_and_stars(shape):
     from slime_b200 import ops

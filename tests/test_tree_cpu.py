@@ -212,6 +212,9 @@ def test_accepted_rows_move_behind_each_other(stacked):
     assert all(torch.equal(a, b) for a, b in zip(caches, want))
 
 
+LATENT = torch.zeros(2, 8, 1, 4)
+
+
 @pytest.mark.parametrize("change, match", [
     (dict(max_nodes=200), "200 nodes"),
     (dict(drafted=torch.zeros(4, dtype=torch.int32)), "drafted"),
@@ -221,6 +224,10 @@ def test_accepted_rows_move_behind_each_other(stacked):
           context_lens=torch.zeros(1, dtype=torch.int32), page_size=4), "one piece"),
     (dict(k_caches=torch.zeros(1, 8, 2, 4), block_table=torch.zeros(2, 2, dtype=torch.int32), context_lens=torch.zeros(1, dtype=torch.int32),
           page_size=4), "block_table"),
+    (dict(k_caches=LATENT, v_caches=LATENT, block_table=torch.zeros(1, 2, dtype=torch.int32), context_lens=torch.zeros(1, dtype=torch.int32), page_size=4),
+     "share memory"),
+    (dict(k_caches=list(LATENT), v_caches=[x[..., :2] for x in LATENT], block_table=torch.zeros(1, 2, dtype=torch.int32),
+          context_lens=torch.zeros(1, dtype=torch.int32), page_size=4), "share memory"),
 ])  # fmt: skip
 def test_acceptance_refuses(change, match):
     z = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
