@@ -30,8 +30,6 @@
 // cleared in shared memory before the product of weights (zero) and values. So are nodes' values that are not finite: rows that see
 // such a node become NaN, and the others stay what they are.
 // Every wait is bounded: on expiry the CTA records a status word, drains and returns with its TMEM freed.
-#include <type_traits>
-
 #include "token_tree.cuh"
 
 namespace sb {
@@ -99,7 +97,7 @@ struct TtArgs {
   const int* parents;
   const float* sinks;
   __nv_bfloat16* out;
-  float* part_o;   // [2 * gridDim][128 * TILES][D]
+  float4* part_o;  // [2 * gridDim][4 * TILES][D / 4][32]: of 32 rows, 4 columns each: a warp has a row per lane, and a store that touches 32 lines takes it 32 cycles
   float2* part_ml;  // [2 * gridDim][128 * TILES]
   int4* plan;      // [gridDim][2]: the item that begins in this CTA and goes on in the next: its parts (0: none) and the first one's slot,
                    // kv head and number of its first node; rows of its tree: first and number
@@ -504,7 +502,6 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       const int tid = threadIdx.x & 127;
       const int copy = row / ROWS, rr = row % ROWS;  // this thread's keys of a tile: columns [copy * COLS, copy * COLS + COLS)
       const int in_tile = rr / a.G, head_in = rr - in_tile * a.G;
-      const int o_rr = tid / REP, o_in = o_rr / a.G, o_head = o_rr - o_in * a.G;  // the row that this thread adds up the copies of
       const uint32_t lane_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
       const uint32_t s_addr = lane_addr + g * TT_BN, o_addr = lane_addr + 2 * TT_BN, p_addr = lane_addr + S::P_COL + g * S::P_STEP;
       const uint64_t c2 = f2_pack(a.c_log2, a.c_log2);
@@ -736,7 +733,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             // a thread writes its row: all of it, or half
             const int col0 = rows2 ? 0 : g * (D / 2), cols = rows2 ? D : D / 2;
             __nv_bfloat16* o_row = a.out + static_cast<long>(walk.r.first + node) * a.out_row + static_cast<long>(walk.kvh * a.G + head_in) * D;
-            float* p_row = a.part_o + (static_cast<long>(slot) * (128 * TILES) + qt * 128 + row) * D;
+            float4* p_row = a.part_o + ((static_cast<long>(slot) * TILES + qt) * 4 + quarter) * (D * 8) + lane;
             const uint32_t mine_o = o_addr + (rows2 ? g * D : 0);
 #pragma unroll 1
             for (int col = col0; col < col0 + cols; col += 16) {
@@ -759,18 +756,20 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
                                                                           pack_bf16x2(v[k + 4], v[k + 5]), pack_bf16x2(v[k + 6], v[k + 7]));
               } else if (valid) {
 #pragma unroll
-                for (int k = 0; k < 16; k += 4) *reinterpret_cast<float4*>(p_row + col + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+                for (int k = 0; k < 16; k += 4) p_row[(col + k) * 8] = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
               }
             }
           }
         } else {
-          // the copies' sums meet in shared memory, 16 columns a turn; then a thread adds up 16 / REP columns of row tid / REP
+          // the copies' sums meet in shared memory, 16 columns a turn; then a thread adds up 16 / REP columns of a row, neighbours of the same
+          // one where rows are written out, of the next one where parts are
           float* mine_red = red + g * (128 * 20);
           constexpr int PER = 16 / REP;
+          const int o_rr = all ? tid / REP : tid % ROWS, o_col = (all ? tid % REP : tid / ROWS) * PER, o_in = o_rr / a.G, o_head = o_rr - o_in * a.G;
           const bool o_valid = ok && o_in < walk.r.n && o_in < a.bq;
-          __nv_bfloat16* o_row = a.out + static_cast<long>(walk.r.first + o_in) * a.out_row + static_cast<long>(walk.kvh * a.G + o_head) * D + (tid % REP) * PER;
-          float* p_row = a.part_o + (static_cast<long>(slot) * 128 + o_rr) * D + (tid % REP) * PER;
-          const float* from = mine_red + o_rr * 20 + (tid % REP) * PER;
+          __nv_bfloat16* o_row = a.out + static_cast<long>(walk.r.first + o_in) * a.out_row + static_cast<long>(walk.kvh * a.G + o_head) * D + o_col;
+          float4* p_row = a.part_o + (static_cast<long>(slot) * 4 + (o_rr >> 5)) * (D * 8) + o_col * 8 + (o_rr & 31);
+          const float* from = mine_red + o_rr * 20 + o_col;
 #pragma unroll 1
           for (int col = g * (D / 2); col < (g + 1) * (D / 2); col += 16) {
             if (ok && active) {
@@ -798,7 +797,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 #pragma unroll
               for (int k = 0; k < PER; k += 4) {
                 if (all) *reinterpret_cast<uint2*>(o_row + col + k) = make_uint2(pack_bf16x2(t[k], t[k + 1]), pack_bf16x2(t[k + 2], t[k + 3]));
-                else *reinterpret_cast<float4*>(p_row + col + k) = make_float4(t[k], t[k + 1], t[k + 2], t[k + 3]);
+                else p_row[(col + k) * 8] = make_float4(t[k], t[k + 1], t[k + 2], t[k + 3]);
               }
             }
             tt_barrier(1 + g, 128);
@@ -827,67 +826,69 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   if (warp == 1) tmem_dealloc(tmem_base, S::TMEM_COLS);
 }
 
-// Joins the parts of items that were split between CTAs: out = sum_p o_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), a warp per row, in the order of the
-// parts. Block x looks at the item that goes on behind CTA x, if there is one.
-constexpr int TT_JOIN_ROWS = 8;
+// Joins the parts of items that were split between CTAs: out = sum_p o_p 2^(m_p - M) / sum_p l_p 2^(m_p - M), in the order of the parts. A lane has a row,
+// a warp every eighth group of 4 columns. Block x looks at the item that goes on behind CTA x, if there is one.
+constexpr int TT_JOIN_THREADS = 256;
 template <int D, int TILES>
-__global__ void __launch_bounds__(32 * TT_JOIN_ROWS)
+__global__ void __launch_bounds__(TT_JOIN_THREADS)
 tree_attn_join_kernel(const __grid_constant__ TtArgs a) {
   pdl_wait();
   pdl_launch_dependents();
-  const int c = blockIdx.x, lane = threadIdx.x & 31;
-  const int x = blockIdx.y * TT_JOIN_ROWS + (threadIdx.x >> 5), row = x & 127, in_tile = row / a.G;
+  const int c = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int x = blockIdx.y * 32 + lane, row = x & 127, in_tile = row / a.G;
   const int4 plan = a.plan[2 * c], tree = a.plan[2 * c + 1];
   const int parts = plan.x, node = plan.w + (x >> 7) * a.bq + in_tile;
-  if (parts == 0 || in_tile >= a.bq || node >= tree.y) return;
-  constexpr int V = D / 32;  // channels of a lane
-  constexpr int FLY = 8;     // parts whose reads are under way together
-  using Vec = typename std::conditional<V == 4, float4, float2>::type;
-  // part p: in slot plan.y, or the first slot of the CTA behind
-  auto at = [&](int p) { return static_cast<long>(p == 0 ? plan.y : 2 * (c + p)) * (128 * TILES) + x; };
-  float top = -INFINITY, l = 0.f, o[V];
+  const bool valid = parts > 0 && in_tile < a.bq && node < tree.y;
+  if (!__any_sync(0xffffffffu, valid)) return;
+  constexpr int NQ = D / 32;         // groups of columns
+  constexpr int FLY = 16 / NQ;       // parts whose reads are under way together
+  float top = -INFINITY, l = 0.f;
+  float4 o[NQ];
   bool hole = false;
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = 0.f;
-  for (int p0 = 0; p0 < parts; p0 += 32) {
-    const int count = min(32, parts - p0);
-    const float2 mine = lane < count ? a.part_ml[at(p0 + lane)] : make_float2(-INFINITY, 0.f);
-    float new_top = 0.f, f = 0.f;
-    for (int p1 = 0; p1 < count; p1 += FLY) {
-      Vec v[FLY];
+  for (int k = 0; k < NQ; ++k) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += FLY) {
+    float2 ml[FLY];
+    float4 v[FLY][NQ];
 #pragma unroll
-      for (int i = 0; i < FLY; ++i)
-        if (p1 + i < count) v[i] = *reinterpret_cast<const Vec*>(a.part_o + at(p0 + p1 + i) * D + lane * V);
-      if (p1 == 0) {  // what was added up so far, and these parts, on the scale of the largest maximum
-        hole = hole || __any_sync(0xffffffffu, mine.y < 0.f);
-        new_top = fmaxf(top, warp_max(mine.x));
-        const float keep = top == -INFINITY ? 0.f : tt_exp2(top - new_top);
-        f = mine.x == -INFINITY ? 0.f : tt_exp2(mine.x - new_top);
-        l = l * keep + warp_sum(mine.y * f);
+    for (int i = 0; i < FLY; ++i) {
+      ml[i] = make_float2(-INFINITY, 0.f);
+      if (valid && p0 + i < parts) {
+        const long slot = p0 + i == 0 ? plan.y : 2 * (c + p0 + i);  // (behind the first part: the first slot of the CTA)
+        ml[i] = a.part_ml[slot * (128 * TILES) + x];
 #pragma unroll
-        for (int k = 0; k < V; ++k) o[k] *= keep;
-        top = new_top;
-      }
-#pragma unroll
-      for (int i = 0; i < FLY; ++i) {
-        const float fp = __shfl_sync(0xffffffffu, f, p1 + i);
-        if (p1 + i < count) {
-          const float* e = reinterpret_cast<const float*>(&v[i]);
-#pragma unroll
-          for (int k = 0; k < V; ++k) o[k] = fmaf(e[k], fp, o[k]);
-        }
+        for (int k = 0; k < NQ; ++k) v[i][k] = a.part_o[(slot * (4 * TILES) + blockIdx.y) * (D * 8) + (warp + 8 * k) * 32 + lane];
       }
     }
+    float new_top = top;
+#pragma unroll
+    for (int i = 0; i < FLY; ++i) new_top = fmaxf(new_top, ml[i].x);
+    const float zero = new_top == -INFINITY ? 0.f : new_top, keep = tt_exp2(top - zero);
+    top = new_top;
+    l *= keep;
+#pragma unroll
+    for (int k = 0; k < NQ; ++k) o[k] = make_float4(o[k].x * keep, o[k].y * keep, o[k].z * keep, o[k].w * keep);
+#pragma unroll
+    for (int i = 0; i < FLY; ++i) {
+      if (!valid || p0 + i >= parts) break;
+      const float f = tt_exp2(ml[i].x - zero);
+      l += ml[i].y * f;
+      hole = hole || ml[i].y < 0.f;
+#pragma unroll
+      for (int k = 0; k < NQ; ++k)
+        o[k] = make_float4(fmaf(v[i][k].x, f, o[k].x), fmaf(v[i][k].y, f, o[k].y), fmaf(v[i][k].z, f, o[k].z), fmaf(v[i][k].w, f, o[k].w));
+    }
   }
+  if (!valid) return;
   const int head = plan.z * a.G + row - in_tile * a.G;
   if (a.sinks != nullptr) l += tt_exp2(a.sinks[head] * 1.4426950408889634f - top);
   const bool some = !hole && l != 0.f;  // (a sum that is NaN comes through)
   const float inv = some ? 1.f / l : 0.f;
+  __nv_bfloat16* dst = a.out + static_cast<long>(tree.x + node) * a.out_row + static_cast<long>(head) * D;
 #pragma unroll
-  for (int k = 0; k < V; ++k) o[k] = some ? o[k] * inv : 0.f;
-  __nv_bfloat16* dst = a.out + static_cast<long>(tree.x + node) * a.out_row + static_cast<long>(head) * D + lane * V;
-  if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-  else *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[0], o[1]);
+  for (int k = 0; k < NQ; ++k)
+    *reinterpret_cast<uint2*>(dst + (warp + 8 * k) * 4) =
+        some ? make_uint2(pack_bf16x2(o[k].x * inv, o[k].y * inv), pack_bf16x2(o[k].z * inv, o[k].w * inv)) : make_uint2(0, 0);
 }
 
 template <int D, int TILES, int REP>
@@ -898,7 +899,7 @@ static int launch_tree_attn(const CUtensorMap& tq, const CUtensorMap& tk, const 
   if (cudaError_t e = launch_pdl(kern, dim3(ctas), dim3(TT_THREADS), S::TOTAL, s, tq, tk, tv, a); e != cudaSuccess) return (int)e;
   if (a.whole) return 0;
   const int rows = TILES == 1 ? a.max_nodes * a.G : 128 * TILES;
-  return (int)launch_pdl(tree_attn_join_kernel<D, TILES>, dim3(ctas, (rows + TT_JOIN_ROWS - 1) / TT_JOIN_ROWS), dim3(32 * TT_JOIN_ROWS), 0, s, a);
+  return (int)launch_pdl(tree_attn_join_kernel<D, TILES>, dim3(ctas, (rows + 31) / 32), dim3(TT_JOIN_THREADS), 0, s, a);
 }
 
 struct TtPlan {
@@ -959,8 +960,8 @@ extern "C" int sb_tree_attn_tc(const void* call, float scale, cudaStream_t s) {
   a.out = reinterpret_cast<__nv_bfloat16*>(x[8]);
   a.plan = reinterpret_cast<int4*>(x[9]);
   a.status = reinterpret_cast<int*>(x[10]);
-  a.part_o = reinterpret_cast<float*>(a.plan + 2l * p.ctas);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + 2l * p.ctas * 128 * p.tiles * D);
+  a.part_o = reinterpret_cast<float4*>(a.plan + 2l * p.ctas);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + 2l * p.ctas * 32 * p.tiles * D);
   a.rows = rows; a.B = B; a.Hkv = Hkv; a.G = Hq / Hkv; a.bq = p.bq; a.page_shift = shift; a.max_pages = max_pages; a.num_slots = num_slots;
   a.max_nodes = max_nodes; a.pairs = p.pairs; a.whole = whole;
   a.out_row = out_row;
