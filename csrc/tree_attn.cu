@@ -101,7 +101,9 @@ extern "C" int sb_tree_attn(const void* q, const void* k_cache, const void* v_ca
                             long v_head, long out_row, float scale, int f32, cudaStream_t s) {
   if (rows <= 0 || B <= 0 || Hq <= 0) return 0;
   if (D > sb::TA_MAXD || D <= 0) return -1;
-  if (Hkv <= 0 || Hq % Hkv != 0 || page_size <= 0 || max_nodes <= 0 || max_nodes > sb::TREE_MAX) return (int)cudaErrorInvalidValue;
+  if (Hkv <= 0 || Hq % Hkv != 0 || page_size <= 0 || max_nodes <= 0 || max_nodes > sb::TREE_MAX || max_pages < 0 ||
+      static_cast<long>(max_pages) * page_size > 0x7fffffffl)
+    return (int)cudaErrorInvalidValue;
   const dim3 grid(rows, (Hq + 3) / 4), block(128);
   if (f32)
     return (int)sb::launch_pdl(sb::tree_attn_kernel<float>, grid, block, 0, s, (const float*)q, (const float*)k_cache, (const float*)v_cache,

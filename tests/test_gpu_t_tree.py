@@ -153,6 +153,27 @@ def test_attention_of_a_long_cache_and_empty_calls():
     assert ops.tree_attention(q[:0], k, v, table[:0], c[:0], none, parents[:0], 16, 12).shape == (0, 8, 128)
 
 
+@pytest.mark.parametrize("page", [16, 24])
+def test_caches_of_more_than_32_bits(page):
+    """The rows in use stand behind 2^31 elements, 2^32 bytes."""
+    from slime_b200 import ops
+
+    heads, sizes, ctx = (16, 8, 64), [9, 17], [150, 33]
+    q, k, v, table, c, cu, parents = attention_case(sizes, ctx, heads, page)
+    first = -(-(1 << 22) // page) * page
+    big = torch.empty(2, 1, first + k.shape[0], 8, 64, dtype=torch.bfloat16, device="cuda")
+    big[0, 0, first:], big[1, 0, first:] = k, v
+    far = table + first // page
+    got = ops.tree_attention(q, big[0, 0], big[1, 0], far, c, cu, parents, page, 17)
+    assert torch.equal(got, ops.tree_attention(q, k, v, table, c, cu, parents, page, 17))
+    sampled, drafted, parents, cu = accept_case(sizes, 2, 1.0)
+    want = oracle.accepted(sampled, drafted, parents, cu, 17)
+    after = oracle.moved([k.cpu()[None], v.cpu()[None]], table.cpu(), ctx, [w[0] for w in want], [w[2] for w in want], page)
+    ops.accept_tree(*cuda(sampled, drafted, parents, cu), 17, k_caches=big[0], v_caches=big[1], block_table=far, context_lens=c, page_size=page)
+    for x, y in zip(big[:, 0, first:].cpu(), after):
+        torch.testing.assert_close(x, y[0], rtol=0, atol=0, equal_nan=True)
+
+
 def test_attention_is_the_same_every_time_and_with_other_requests_beside_it_where_asked():
     from slime_b200 import ops
 
