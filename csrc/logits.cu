@@ -138,6 +138,8 @@ __device__ __forceinline__ void lg_text(const LogitsArgs& a, int req, int thread
   }
 }
 
+__device__ __forceinline__ void lg_prefetch(const void* at) { asm volatile("prefetch.global.L1 [%0];" ::"l"(at)); }
+
 // ---------------------------------------------------------------- one launch: CHUNK tokens of a row, CHUNK / 256 a thread
 template <typename T, int CHUNK>
 __global__ void __launch_bounds__(LG_THREADS)
@@ -279,12 +281,20 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
   const float rep = a.repetition != nullptr ? a.repetition[req] : 1.f;
   const float freq = a.frequency != nullptr ? a.frequency[req] : 0.f;
   const float pres = a.presence != nullptr ? a.presence[req] : 0.f;
-  const bool counts = a.penal && (rep != 1.f || freq != 0.f || pres != 0.f);
+  // (read whether they count or not: one wait for memory instead of two)
+  const int all_len = a.penal ? max(min(a.lengths[req], a.text), 0) : 0, all_prompt = a.penal && a.prompts != nullptr ? a.prompts[req] : 0;
   const int K = a.biases;
   const int* ids = a.bias_ids + req * a.bias_row;
   const float* values = a.bias_values + req * a.bias_row;
-  const int len = counts ? max(min(a.lengths[req], a.text), 0) : 0;
-  const int prompt = counts && a.prompts != nullptr ? a.prompts[req] : 0;
+  if (tid < K) {
+    lg_prefetch(ids + tid);
+    lg_prefetch(values + tid);
+  }
+  const bool counts = a.penal && (rep != 1.f || freq != 0.f || pres != 0.f);
+  const int len = counts ? all_len : 0, prompt = counts ? all_prompt : 0;
+#pragma unroll
+  for (int x = 0; x < LG_FLY; ++x)
+    if (tid + x * THREADS < len) lg_prefetch(a.tokens + req * a.tokens_row + tid + x * THREADS);
   const bool direct = static_cast<long>(len) + K + n > HASH / 4 * 3;
   for (int i = tid; i < n; i += THREADS) {
     tree_p[i] = a.parents[first + i];

@@ -21,8 +21,8 @@ def check(sampling, rows: int = 1):
 
 
 def adjust(logits, reqs, chains=None):
-    """Logits of ``reqs`` adjusted in place, a row for each; nothing happens if no request asks. ``chains`` = (ids, cu): request b has the rows cu[b] .. cu[b + 1]
-    for the last token of its text and the guesses behind it, which the device tensors ``ids`` and ``cu`` name."""
+    """Logits of ``reqs`` adjusted in place, a row for each; nothing happens if no request asks. ``chains`` = (ids, cu), device tensors: request b
+    has the rows cu[b] .. cu[b + 1], for the last token of its text and the guesses behind it, which ``ids`` names."""
     if not any(r.sampling.adjusts for r in reqs):
         return logits
     dev, B = logits.device, len(reqs)

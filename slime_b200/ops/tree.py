@@ -124,8 +124,8 @@ def tree_attention(q, k_cache, v_cache, block_table, context_lens, cu_nodes, par
     a value. ``max_nodes``: no tree has more nodes. Rows of ``out`` behind ``cu_nodes[B]`` are left as they are (a new ``out``: undefined).
 
     What a row does not see may be anything, NaN too: other branches, nodes of no tree, the rest of a page. A row that sees a value that
-    is not finite, with a weight above zero, has no finite output (of a node: its head is NaN as a whole). bf16, and fp32 throughout; heads up to 256 wide. In batch-invariant mode a row's
-    bits depend on its own tree and ``max_nodes``, not on the requests beside it."""
+    is not finite, with a weight above zero, has no finite output (of a node: its head is NaN as a whole). bf16, and fp32 throughout;
+    heads up to 256 wide. In batch-invariant mode a row's bits depend on its own tree and ``max_nodes``, not on the requests beside it."""
     kv, dev, dtype, B = k_cache.shape, q.device, q.dtype, context_lens.shape[0]
     # (one expression for calls that are in order, which is most of what a call costs on the host; the check proper says what is wrong with others)
     if not (q.dim() == 3 and len(kv) == 3 and v_cache.shape == kv and kv[2] == q.shape[2] <= 256 and kv[1] > 0 and q.shape[1] % kv[1] == 0 and page_size > 0
