@@ -12,7 +12,7 @@
 // Biases of a token are added up in list order by one thread: nothing depends on an order of arrival. Logits that the mask hides are not read.
 // Everything is worked out in fp32 and rounded once. What bounds it: reading and writing the logits, 16 bytes a thread and access; a row that
 // does not start on such a boundary is cut at the boundaries all the same, and its two ends go element by element.
-// Measured (B200): 256 rows of 151936 fp32, texts of 1150: 70 us, of which the rows take 46 (6.8 TB/s) and counting, a chain of atomics and loads in few CTAs, the
+// Measured (B200): 256 rows of 151936 fp32, texts of 1150: 64 us, of which the rows take 46 (6.8 TB/s) and counting, a chain of atomics and loads in few CTAs, the
 // rest; 763 rows of 61 trees with masks: 172 us, 0.81 of the copy rate; one row: 3.9 us.
 #include "token_tree.cuh"
 
@@ -122,7 +122,7 @@ __device__ __forceinline__ float lg_used(float v, bool seen, int times, float re
 
 // What there is of a token: in the prompt, has a bias, was drafted, and how many times it was answered with. lg_text: each token of a request's text.
 enum : int { LG_PROMPT = 1 << 30, LG_BIAS = 1 << 29, LG_DRAFT = 1 << 28 };
-constexpr int LG_FLY = 8;  // tokens whose reads are under way together
+constexpr int LG_FLY = 4;  // tokens whose reads are under way together
 template <typename F>
 __device__ __forceinline__ void lg_text(const LogitsArgs& a, int req, int threads, const F& each) {
   const int* text = a.tokens + req * a.tokens_row;
@@ -260,10 +260,9 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
 // ---------------------------------------------------------------- two launches: count; then copy, mask and put in what was counted
 // Lists the tokens of a request that were used, drafted or have a bias, by bucket of the vocabulary. They are counted in a hash table of HASH places
 // in shared memory (linear probing, at most three quarters full); a longer text is counted in a table of 2 HASH tokens of the vocabulary at a time.
-template <int HASH>
-__global__ void __launch_bounds__(HASH / 16, HASH == 8192 ? 2 : 1)
+template <int HASH, int THREADS>
+__global__ void __launch_bounds__(THREADS, HASH == 8192 ? 2 : 1)
 logits_count_kernel(const __grid_constant__ LogitsArgs a) {
-  constexpr int THREADS = HASH / 16;
   extern __shared__ __align__(16) int tables[];
   int* keys = tables;          // [HASH] token, -1: empty
   int* hashed = tables + HASH;  // [HASH] what there is of it
@@ -346,7 +345,7 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
       if (direct) return t >= base && t - base < 2 * HASH ? tables + (t - base) : nullptr;
       return &hashed[probe(t, hash(t), came)];
     };
-    uint32_t brought = 0, brought_x = 0;  // of this thread's tokens of the text, one bit each (at most 16); of drafted nodes and biases
+    uint32_t brought = 0, brought_x = 0;  // of this thread's tokens of the text, one bit each (at most 12); of drafted nodes and biases
     bool came;
     if (counts) {
       int batch = 0;
@@ -477,7 +476,7 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
     }
     if (pass + 1 < passes) __syncthreads();
   }
-  pdl_launch_dependents();  // not before: rows that wait for the lists would slow the counting down (72 us for 256 rows of 151936, 66 so)
+  pdl_launch_dependents();  // not before: rows that wait for the lists would slow the counting down (a tenth of the call at 256 rows of 151936)
 }
 
 // Copies and masks a chunk of a row, then puts in the logits of the listed tokens (their lines have just been here).
@@ -578,11 +577,11 @@ static long lg_lists(LogitsArgs& a, void* work, int sms) {
 // Small calls: everything in one launch, 8 tokens a thread.
 static bool lg_small(const LogitsArgs& a, int sms) { return static_cast<long>((a.vocab + 7 + 2047) / 2048) * a.rows <= 8L * sms; }
 
-template <int HASH>
+template <int HASH, int THREADS>
 static cudaError_t launch_count(const LogitsArgs& a, cudaStream_t s) {
-  auto kern = logits_count_kernel<HASH>;
+  auto kern = logits_count_kernel<HASH, THREADS>;
   if (cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kern), 2 * HASH * 4); e != cudaSuccess) return e;
-  return launch_pdl(kern, dim3(a.requests * a.lists), dim3(HASH / 16), 2 * HASH * 4, s, a);
+  return launch_pdl(kern, dim3(a.requests * a.lists), dim3(THREADS), 2 * HASH * 4, s, a);
 }
 
 template <typename T>
@@ -595,8 +594,12 @@ static int launch_logits(LogitsArgs a, void* work, long work_bytes, int sms, cud
       return (int)launch_pdl(logits_kernel<T, 2048>, dim3(a.chunks * a.rows), dim3(LG_THREADS), 0, s, a);
     }
     if (lg_lists(a, work, sms) > work_bytes) return (int)cudaErrorInvalidValue;
-    // 64 KB of table leave room for three CTAs on an SM, 128 KB take a text of 12,000 tokens
-    const cudaError_t e = static_cast<long>(a.text) + a.biases + TREE_MAX <= 6144 ? launch_count<8192>(a, s) : launch_count<16384>(a, s);
+    // 64 KB of table leave room for two CTAs on an SM, 128 KB take a text of 12,000 tokens. A token's turn is a chain of looks at the table, so texts of some
+    // length want more threads (256 texts of 257 to 2047: 64.4 us for the call with 1024 threads, 69.6 with 512); 512 requests with biases alone: 27.7 and 22.9.
+    const bool wide = a.text > 1024;
+    const cudaError_t e = static_cast<long>(a.text) + a.biases + TREE_MAX > 6144 ? launch_count<16384, 1024>(a, s)
+                          : wide                                                   ? launch_count<8192, 1024>(a, s)
+                                                                                   : launch_count<8192, 512>(a, s);
     if (e != cudaSuccess) return (int)e;
     a.listed = 1;
   }
