@@ -6,6 +6,8 @@ Requests that ask for nothing pass through untouched, and a batch in which nobod
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from slime_b200 import ops
@@ -16,8 +18,13 @@ def check(sampling, rows: int = 1):
     """Raises ValueError on penalties that have no meaning, and where a pass has more ``rows`` for a request than a tree of the operator has nodes."""
     if sampling.adjusts and rows > tree_ops.MAX_NODES:
         raise ValueError(f"penalties take chains of at most {tree_ops.MAX_NODES - 1} guesses, not {rows - 1}")
-    if not sampling.repetition_penalty > 0:
+    if not 0 < sampling.repetition_penalty < math.inf:
         raise ValueError(f"repetition_penalty must be above zero, not {sampling.repetition_penalty}")
+    if not (math.isfinite(sampling.frequency_penalty) and math.isfinite(sampling.presence_penalty)):
+        raise ValueError(f"frequency_penalty {sampling.frequency_penalty}, presence_penalty {sampling.presence_penalty}: must be numbers")
+    for token, value in (sampling.logit_bias or {}).items():
+        if not isinstance(token, int) or not 0 <= token < 1 << 31 or not value < math.inf:
+            raise ValueError(f"logit_bias: {value} for token {token!r}")
 
 
 def adjust(logits, reqs, chains=None):

@@ -77,6 +77,14 @@ def test_penalties_as_they_arrive():
     assert SamplingParams.from_dict(dict(logit_bias={"12": -3})).logit_bias == {12: -3.0}
     assert EngineServer._openai_sampling(dict(frequency_penalty=0.5, presence_penalty=1, logit_bias={"3": 1}))["frequency_penalty"] == 0.5
     _, _, plain, _ = _pair("dense")
-    for bad in (0, -1.0, float("nan")):
-        with pytest.raises(ValueError, match="repetition_penalty"):
-            plain.add_request([1, 2], dict(repetition_penalty=bad))
+    nan, inf = float("nan"), float("inf")
+    for name, values in (("repetition_penalty", (0, -1.0, nan, inf)), ("frequency_penalty", (nan, inf)), ("presence_penalty", (nan, -inf)),
+                         ("logit_bias", ({-1: 1.0}, {1 << 31: 1.0}, {3: nan}, {3: inf}))):  # fmt: skip
+        for bad in values:
+            with pytest.raises(ValueError, match=name):
+                plain.add_request([1, 2], {name: bad})
+    with pytest.raises(ValueError, match="logit_bias"):
+        plain.add_request([1, 2], SamplingParams(logit_bias={"3": 1.0}))
+    assert not plain.has_work()
+    none = plain.generate([[1, 2, 3]], dict(max_new_tokens=4, temperature=0, ignore_eos=True, logit_bias={t: -inf for t in range(40)}))[0]
+    assert min(none.output_ids) >= 40
