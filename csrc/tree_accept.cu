@@ -20,7 +20,7 @@ constexpr int AC_SLABS = 128;
 struct AcceptSlabs {
   uint8_t* base[AC_SLABS];  // each the first of `layers` slabs, `step` bytes apart
   long step;
-  int layers, count, slots, row_units, unit;  // slabs in all; a row: row_units pieces of `unit` bytes (2, 4, 8 or 16)
+  int layers, count, slots, row_units, unit;  // slabs in all; a row: row_units pieces of `unit` bytes (1, 2, 4, 8 or 16)
   long row_bytes;           // pitch of a slot
 };
 
@@ -123,15 +123,16 @@ tree_accept_kernel(const int* __restrict__ sampled, const int* __restrict__ draf
   if (slabs.unit == 16) accept_move<uint4>(slabs, src, dst, moves, blockIdx.y, gridDim.y);
   else if (slabs.unit == 8) accept_move<uint2>(slabs, src, dst, moves, blockIdx.y, gridDim.y);
   else if (slabs.unit == 4) accept_move<uint32_t>(slabs, src, dst, moves, blockIdx.y, gridDim.y);
-  else accept_move<uint16_t>(slabs, src, dst, moves, blockIdx.y, gridDim.y);
+  else if (slabs.unit == 2) accept_move<uint16_t>(slabs, src, dst, moves, blockIdx.y, gridDim.y);
+  else accept_move<uint8_t>(slabs, src, dst, moves, blockIdx.y, gridDim.y);
 }
 
 }  // namespace sb
 
 // call: addresses of sampled, drafted, parents, cu, path, tokens, count, page table and context lengths; then rows, B, most nodes, page size, pages of a row
 // of the table, whether to write path, tokens and count, SMs, slabs behind each address, bytes between them, slots, pieces of a row, bytes of a
-// piece (2, 4, 8 or 16), bytes from one slot to the next, number of addresses, and the addresses, each the first of so many slabs. path, tokens:
-// [B, max_nodes], -1 behind the accepted nodes; count: [B]. No address: nothing is moved.
+// piece (1, 2, 4, 8 or 16; addresses and pitches are multiples of it), bytes from one slot to the next, number of addresses, and the addresses, each the first of
+// so many slabs. path, tokens: [B, max_nodes], -1 behind the accepted nodes; count: [B]. No address: nothing is moved.
 extern "C" int sb_tree_accept(const void* call, cudaStream_t s) {
   const long long* x = static_cast<const long long*>(call);
   auto ints = [&](int i) { return reinterpret_cast<int*>(x[i]); };
@@ -147,6 +148,11 @@ extern "C" int sb_tree_accept(const void* call, cudaStream_t s) {
   c.row_units = static_cast<int>(x[19]);
   c.unit = static_cast<int>(x[20]);
   c.row_bytes = x[21];
+  if (n > 0) {
+    bool fits = c.unit > 0 && c.unit <= 16 && (c.unit & (c.unit - 1)) == 0 && c.row_bytes % c.unit == 0 && c.step % c.unit == 0;
+    for (int i = 0; i < n; ++i) fits = fits && x[23 + i] % c.unit == 0;
+    if (!fits) return (int)cudaErrorInvalidValue;
+  }
   const long all = (static_cast<long>(c.count) * c.row_units + sb::AC_THREADS - 1) / sb::AC_THREADS;
   const long want = (4L * sms + B - 1) / B;
   const int parts = static_cast<int>(all < 1 ? 1 : (all < want ? all : want));

@@ -458,6 +458,33 @@ def test_acceptance_of_many_layers_in_a_list_and_empty_values():
     assert path.shape == (0, 4) and count.shape == (0,)
 
 
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("H, D, left", [(1, 1, 0), (1, 3, 0), (2, 4, 0), (3, 16, 0), (1, 6, 1), (3, 5, 2), (1, 16, 4)])
+def test_acceptance_of_one_byte_caches(dtype, H, D, left):
+    """Rows of odd and even numbers of bytes, from odd and even addresses (``left`` bytes into a wider row): only the rows of the path change, and nothing
+    between or behind them."""
+    from slime_b200 import ops
+
+    sizes, ctx = [9, 1, 40], [15, 3, 2]
+    sampled, drafted, parents, cu = accept_case(sizes, 4, 1.0)
+    table, slots = oracle.make_pages([c + n for c, n in zip(ctx, sizes)], 16, 1)
+    want = oracle.accepted(sampled, drafted, parents, cu, 40)
+    g = torch.Generator().manual_seed(D)
+    for wide in (H * D + left, H * D + left + 3):  # a row's pitch
+        store = torch.randint(0, 120, (2, 3, slots, wide), generator=g, dtype=torch.uint8)
+        view = lambda t: t[..., left : left + H * D].unflatten(-1, (H, D))  # noqa: E731
+        after = store.clone()
+        for s in range(2):
+            moved = oracle.moved([view(store[s]).contiguous()], table, ctx, [w[0] for w in want], [w[2] for w in want], 16)[0]
+            view(after[s]).copy_(moved)
+        for split in (False, True):
+            dev = store.cuda()
+            k, v = (view(dev[s]).view(dtype) for s in range(2))
+            ops.accept_tree(*cuda(sampled, drafted, parents, cu), 40, k_caches=list(k) if split else k, v_caches=list(v) if split else v,
+                            block_table=table.cuda(), context_lens=torch.tensor(ctx, dtype=torch.int32, device="cuda"), page_size=16)  # fmt: skip
+            assert torch.equal(dev.cpu(), after)
+
+
 # ------------------------------------------------------------------------------------------------------- a whole round
 def test_a_round_of_drafted_trees_is_ordinary_decoding():
     """One attention layer with a vocabulary behind it, in fp32 (close calls of the sampler aside, both forms then draw the same tokens): two rounds of trees, penalties included,

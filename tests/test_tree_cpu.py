@@ -234,3 +234,28 @@ def test_acceptance_refuses(change, match):
     args = dict(sampled=z(3), drafted=z(3), parents=z(3), cu_nodes=torch.tensor([0, 3], dtype=torch.int32), max_nodes=3)
     with pytest.raises(ValueError, match=match):
         ops.accept_tree(**{**args, **change})
+
+
+def test_the_entry_of_acceptance_moves_rows_in_pieces_that_fit():
+    """Pieces are 1, 2, 4, 8 or 16 bytes, and addresses and pitches are multiples of them; the entry refuses any other call before it launches anything."""
+    from slime_b200.ops import _lib, tree
+
+    if not _lib.available():
+        pytest.skip("the kernel library is not built")
+    fn, invalid = _lib.lib().sb_tree_accept, 1  # cudaErrorInvalidValue
+    # (unit, bytes from slot to slot, bytes from slab to slab, address)
+    for unit, pitch, step, base in ((3, 3, 0, 48), (0, 16, 0, 48), (-1, 16, 0, 48), (32, 32, 0, 64), (2, 3, 0, 48), (2, 4, 5, 48), (2, 4, 0, 49)):
+        call = tree._ACCEPT(*[0] * 9, 4, 1, 4, 1, 1, 1, 148, 1, step, 8, 3, unit, pitch, 1) + base.to_bytes(8, "little")
+        assert fn(call, None) == invalid
+
+
+@pytest.mark.parametrize("width", [1, 3, 6])
+def test_accepted_rows_of_one_byte_elements(width):
+    sampled, drafted, parents, cu = accept_case([9, 4], 3)
+    ctx = [5, 11]
+    table, slots = oracle.make_pages([c + n for c, n in zip(ctx, [9, 4])], 4, 0)
+    caches = [torch.randint(0, 256, (2, slots, 1, width), dtype=torch.uint8)]
+    want = oracle.accepted(sampled, drafted, parents, cu, 9)
+    after = oracle.moved(caches, table, ctx, [w[0] for w in want], [w[2] for w in want], 4)
+    ops.accept_tree(sampled, drafted, parents, cu, 9, k_caches=caches[0], block_table=table, context_lens=torch.tensor(ctx, dtype=torch.int32), page_size=4)
+    assert torch.equal(caches[0], after[0])
