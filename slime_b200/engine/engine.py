@@ -172,9 +172,13 @@ class Engine:
             self.kv.allocator.refcnt[0] = 1
 
     # ------------------------------------------------------------------ intake
+    def check_sampling(self, sp: SamplingParams):
+        """Raises ValueError on what a request cannot be sampled with."""
+        penalties.check(sp, self.cfg.vocab_size, rows=1 if self.spec is None else self.spec.k + 1)
+
     def add_request(self, input_ids, sampling: SamplingParams | dict | None = None, rid: str | None = None, **kw) -> Request:
         sp = sampling if isinstance(sampling, SamplingParams) else SamplingParams.from_dict(sampling)
-        penalties.check(sp, rows=1 if self.spec is None else self.spec.k + 1)
+        self.check_sampling(sp)
         req = Request(rid=rid or uuid.uuid4().hex, input_ids=list(input_ids), sampling=sp, **kw)
         # Without an explicit seed the stream is numbered by arrival order: the ranks of a tensor-parallel engine see the
         # same requests in the same order, so they draw the same tokens (a hash of the random request id would differ
@@ -531,7 +535,7 @@ class Engine:
         if self.runner.recurrent:
             raise NotImplementedError("prefill / decode disaggregation does not carry the recurrent state of a request")
         sp = sampling if isinstance(sampling, SamplingParams) else SamplingParams.from_dict(sampling)
-        penalties.check(sp)
+        self.check_sampling(sp)
         req = Request(rid=rid or uuid.uuid4().hex, input_ids=list(input_ids), sampling=sp, **kw)
         self._req_counter = getattr(self, "_req_counter", 0) + 1
         req.seed = sp.sampling_seed if sp.sampling_seed is not None else (self.args.random_seed * 1000003 + self._req_counter) & 0x7FFFFFFFFFFF

@@ -14,17 +14,28 @@ from slime_b200 import ops
 from slime_b200.ops import tree as tree_ops
 
 
-def check(sampling, rows: int = 1):
-    """Raises ValueError on penalties that have no meaning, and where a pass has more ``rows`` for a request than a tree of the operator has nodes."""
+# Penalties and biases are worked out in fp32: up to this size (a repetition penalty: and down to its inverse) a count of 2^24 tokens times a penalty, a bias
+# behind it and a temperature of 1e-10 stay within its range, and a logit is never zero times or divided by zero.
+LARGEST = 1e9
+
+
+def check(sampling, vocab: int, rows: int = 1):
+    """Raises ValueError on penalties that have no meaning or none in fp32, on biases that leave no token of the ``vocab``, and where a pass has more ``rows`` for a
+    request than a tree of the operator has nodes."""
     if sampling.adjusts and rows > tree_ops.MAX_NODES:
         raise ValueError(f"penalties take chains of at most {tree_ops.MAX_NODES - 1} guesses, not {rows - 1}")
-    if not 0 < sampling.repetition_penalty < math.inf:
-        raise ValueError(f"repetition_penalty must be above zero, not {sampling.repetition_penalty}")
-    if not (math.isfinite(sampling.frequency_penalty) and math.isfinite(sampling.presence_penalty)):
-        raise ValueError(f"frequency_penalty {sampling.frequency_penalty}, presence_penalty {sampling.presence_penalty}: must be numbers")
+    if not 1 / LARGEST <= sampling.repetition_penalty <= LARGEST:
+        raise ValueError(f"repetition_penalty must be from {1 / LARGEST:g} to {LARGEST:g}, not {sampling.repetition_penalty}")
+    for name in ("frequency_penalty", "presence_penalty"):
+        if not abs(getattr(sampling, name)) <= LARGEST:
+            raise ValueError(f"{name} must be a number of at most {LARGEST:g} either way, not {getattr(sampling, name)}")
+    hidden = 0
     for token, value in (sampling.logit_bias or {}).items():
-        if not isinstance(token, int) or not 0 <= token < 1 << 31 or not value < math.inf:
-            raise ValueError(f"logit_bias: {value} for token {token!r}")
+        if not isinstance(token, int) or not 0 <= token < 1 << 31 or not (abs(value) <= LARGEST or value == -math.inf):
+            raise ValueError(f"logit_bias: {value} for token {token!r} (a number of at most {LARGEST:g} either way, or minus infinity)")
+        hidden += token < vocab and value == -math.inf
+    if hidden >= vocab:
+        raise ValueError("logit_bias: no token of the vocabulary is left")
 
 
 def adjust(logits, reqs, chains=None):

@@ -88,3 +88,34 @@ def test_penalties_as_they_arrive():
     assert not plain.has_work()
     none = plain.generate([[1, 2, 3]], dict(max_new_tokens=4, temperature=0, ignore_eos=True, logit_bias={t: -inf for t in range(40)}))[0]
     assert min(none.output_ids) >= 40
+
+
+@pytest.mark.parametrize("name, bad", [
+    ("repetition_penalty", 1e-46), ("repetition_penalty", 1e-30), ("repetition_penalty", 1e39), ("repetition_penalty", 2e38), ("frequency_penalty", -3e38),
+    ("frequency_penalty", 1e39), ("presence_penalty", -1e39), ("presence_penalty", 3e38), ("logit_bias", {5: 1e39}), ("logit_bias", {5: 3e38}),
+    ("logit_bias", {5: -3e38}),
+])  # fmt: skip
+def test_penalties_that_leave_no_distribution_in_fp32_are_refused(name, bad):
+    """Numbers of 64 bits that fp32 rounds to zero or infinity, or that run over when they are counted or added, are no penalties; a running request goes on."""
+    _, _, plain, spec = _pair("dense")
+    for engine in (plain, spec):
+        with pytest.raises(ValueError, match=name):
+            engine.add_request([1, 2, 3], dict(max_new_tokens=4, temperature=0, ignore_eos=True, **{name: bad}))
+        assert not engine.has_work()
+
+
+def test_the_largest_penalties_still_leave_a_distribution():
+    _, _, plain, _ = _pair("dense")
+    V, inf = plain.cfg.vocab_size, float("inf")
+    base = dict(max_new_tokens=8, ignore_eos=True)
+    asks = [dict(frequency_penalty=s * 1e9, presence_penalty=s * 1e9, repetition_penalty=r, logit_bias={5: s * 1e9, 6: -s * 1e9, 7: -inf})
+            for s in (-1, 1) for r in (1e-9, 1e9)]  # fmt: skip
+    for temperature in (0, 1.0, 0.01):
+        for r in plain.generate([[1, 2, 3]] * len(asks), [dict(base, temperature=temperature, **a) for a in asks]):
+            assert len(r.output_ids) == 8 and 7 not in r.output_ids and np.isfinite(r.output_logprobs).all()
+    # no token is left: refused, one is: taken
+    with pytest.raises(ValueError, match="logit_bias"):
+        plain.add_request([1, 2, 3], dict(base, logit_bias={t: -inf for t in range(V + 3)}))
+    assert not plain.has_work()
+    one = plain.generate([[1, 2, 3]], dict(base, logit_bias={t: -inf for t in range(V + 3) if t != 9}))[0]
+    assert one.output_ids == [9] * 8
