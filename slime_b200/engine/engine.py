@@ -986,8 +986,10 @@ class Engine:
                  **kw) -> list[Request]:
         if not isinstance(sampling, list):
             sampling = [sampling] * len(prompts)
-        reqs = [self.add_request(p, SamplingParams.from_dict(s) if isinstance(s, dict) or s is None else s, **kw)
-                for p, s in zip(prompts, sampling)]  # fmt: skip
+        sampling = [SamplingParams.from_dict(s) if isinstance(s, dict) or s is None else s for s in sampling]
+        for sp in sampling:  # all of them, before any request is queued
+            self.check_sampling(sp)
+        reqs = [self.add_request(p, s, **kw) for p, s in zip(prompts, sampling)]
         while any(not r.finished() for r in reqs):
             if not self.has_work():
                 break

@@ -104,6 +104,16 @@ class EngineServer:
             ids = expand_image_placeholders(ids, cfg.video_token_id, counts)
         return ids, mm
 
+    def _sampling(self, given: list[dict]) -> list[SamplingParams]:
+        """Sampling parameters of all requests of a body, before any of them is queued; ValueError on what cannot be sampled with."""
+        try:
+            out = [SamplingParams.from_dict(s) for s in given]
+            for sp in out:
+                self.engine.check_sampling(sp)
+        except (TypeError, AttributeError, OverflowError) as e:  # (a text or a list where a number or an object belongs)
+            raise ValueError(f"sampling parameters: {e}") from e
+        return out
+
     async def _generate(self, request):
         from aiohttp import web
 
@@ -123,7 +133,10 @@ class EngineServer:
         batched = bool(ids) and isinstance(ids[0], list)
         prompts = ids if batched else [ids]
         sp = body.get("sampling_params") or {}
-        sps = sp if isinstance(sp, list) else [sp] * len(prompts)
+        try:
+            sps = self._sampling(sp if isinstance(sp, list) else [sp] * len(prompts))
+        except ValueError as e:
+            return web.json_response({"error": str(e)}, status=400)
         loop = asyncio.get_running_loop()
         stream = bool(body.get("stream"))
         prefill_only = body.get("disaggregation") == "prefill"
@@ -147,7 +160,7 @@ class EngineServer:
                     loop.call_soon_threadsafe(q.put_nowait, len(r.output_ids))
 
             req = self.engine.add_request(
-                p, SamplingParams.from_dict(s), rid=body.get("rid"), return_logprob=bool(body.get("return_logprob", False)),
+                p, s, rid=body.get("rid"), return_logprob=bool(body.get("return_logprob", False)),
                 logprob_start_len=int(body.get("logprob_start_len", -1) if body.get("return_logprob") else -1),
                 return_routed_experts=bool(body.get("return_routed_experts", False)), stream=stream,
                 on_token=on_token if stream else None, done_event=_Done(ev), prefill_only=prefill_only, mm=mm,
@@ -199,7 +212,7 @@ class EngineServer:
         raw = lambda t: t.view(torch.uint8).numpy().tobytes()  # noqa: E731
         return web.Response(body=len(header).to_bytes(4, "little") + header + raw(k) + raw(v), content_type="application/octet-stream")
 
-    async def _generate_imported(self, body, ids, sampling, room):
+    async def _generate_imported(self, body, ids, sampling: SamplingParams, room):
         """Decode side: pull the KV from the prefill worker named in the request and continue from its first token."""
         import aiohttp
         from aiohttp import web
@@ -234,8 +247,7 @@ class EngineServer:
 
         try:
             req = self.engine.import_request(ids, int(body["first_token"]), float(body.get("first_logprob", 0.0)), (k, v),
-                                             SamplingParams.from_dict(sampling), rid=body.get("rid"),
-                                             return_logprob=bool(body.get("return_logprob", False)), done_event=_Done())  # fmt: skip
+                                             sampling, rid=body.get("rid"), return_logprob=bool(body.get("return_logprob", False)), done_event=_Done())  # fmt: skip
         except Exception as e:  # noqa: BLE001 - out of pages, shape mismatch
             return web.json_response({"error": repr(e)}, status=503)
         mb = len(blob) / 1e6
@@ -249,7 +261,7 @@ class EngineServer:
         return web.json_response(self._render(req))
 
     # ---------------------------------------------------------------- OpenAI-compatible front end
-    async def _run_one(self, ids: list[int], sampling: dict, rid=None):
+    async def _run_one(self, ids: list[int], sampling: SamplingParams, rid=None):
         """Submit one request and wait for it (shared by the chat and completion endpoints)."""
         loop = asyncio.get_running_loop()
         ev = asyncio.Event()
@@ -258,7 +270,7 @@ class EngineServer:
             def set(self_inner):
                 loop.call_soon_threadsafe(ev.set)
 
-        req = self.engine.add_request(ids, SamplingParams.from_dict(sampling), rid=rid, return_logprob=False, done_event=_Done())
+        req = self.engine.add_request(ids, sampling, rid=rid, return_logprob=False, done_event=_Done())
         if req.finished():
             ev.set()
         self._wake.set()
@@ -297,7 +309,11 @@ class EngineServer:
         else:
             text = self.tokenizer.apply_chat_template(messages, tokenize=False, add_generation_prompt=True, **kw)
         ids = self.tokenizer.encode(text, add_special_tokens=False)
-        req = await self._run_one(ids, self._openai_sampling(body), rid=body.get("rid"))
+        try:
+            (sampling,) = self._sampling([self._openai_sampling(body)])
+        except ValueError as e:
+            return web.json_response({"error": {"message": str(e)}}, status=400)
+        req = await self._run_one(ids, sampling, rid=body.get("rid"))
         content = self.tokenizer.decode(req.output_ids, skip_special_tokens=True)
         return web.json_response({
             "id": f"chatcmpl-{req.rid}", "object": "chat.completion", "created": int(time.time()),
@@ -315,7 +331,11 @@ class EngineServer:
         if prompt is None or (isinstance(prompt, str) and self.tokenizer is None):
             return web.json_response({"error": {"message": "prompt (token ids, or text with a tokenizer) is required"}}, status=400)
         ids = self.tokenizer.encode(prompt, add_special_tokens=False) if isinstance(prompt, str) else list(prompt)
-        req = await self._run_one(ids, self._openai_sampling(body), rid=body.get("rid"))
+        try:
+            (sampling,) = self._sampling([self._openai_sampling(body)])
+        except ValueError as e:
+            return web.json_response({"error": {"message": str(e)}}, status=400)
+        req = await self._run_one(ids, sampling, rid=body.get("rid"))
         text = self.tokenizer.decode(req.output_ids, skip_special_tokens=True) if self.tokenizer is not None else ""
         return web.json_response({
             "id": f"cmpl-{req.rid}", "object": "text_completion", "created": int(time.time()),

@@ -119,3 +119,32 @@ def test_the_largest_penalties_still_leave_a_distribution():
     assert not plain.has_work()
     one = plain.generate([[1, 2, 3]], dict(base, logit_bias={t: -inf for t in range(V + 3) if t != 9}))[0]
     assert one.output_ids == [9] * 8
+
+
+def test_a_refused_penalty_is_a_client_error_and_nothing_of_its_body_is_queued():
+    import requests
+
+    engine = make_engine()
+    srv = EngineServer(engine, "127.0.0.1", 0).start(block=False)
+    try:
+        url = f"http://127.0.0.1:{srv.port}"
+        post = lambda path, **body: requests.post(url + path, json=body, timeout=60)  # noqa: E731
+        good = dict(max_new_tokens=100, ignore_eos=True)
+        for bad in (dict(repetition_penalty=0), dict(frequency_penalty=-3e38), dict(logit_bias={"x": 1}), dict(logit_bias=[1, 2]), dict(presence_penalty="much"),
+                    dict(repetition_penalty=[1]), dict(logit_bias={"5": None}), dict(frequency_penalty=10**400)):  # fmt: skip
+            steps = engine.stats["steps"]
+            r = post("/generate", input_ids=[[1, 2], [3, 4], [5]], sampling_params=[good, dict(good, **bad), good])
+            assert r.status_code == 400 and r.json()["error"], r.text
+            assert post("/generate", input_ids=[1, 2], sampling_params=dict(good, **bad)).status_code == 400
+            r = post("/generate", input_ids=[1, 2], sampling_params=dict(good, **bad), bootstrap_room="r", bootstrap_host="http://127.0.0.1:1", first_token=3)
+            assert r.status_code == 400  # (before the keys and values are fetched)
+            r = post("/v1/completions", prompt=[1, 2, 3], max_tokens=100, **bad)
+            assert r.status_code == 400 and r.json()["error"]["message"]
+            assert not engine.has_work() and engine.stats["steps"] == steps
+        r = post("/v1/completions", prompt=[1, 2, 3], max_tokens=5, temperature=0, frequency_penalty=0.5, logit_bias={"7": -100})
+        assert r.status_code == 200 and r.json()["usage"]["completion_tokens"] == 5
+    finally:
+        srv.shutdown()
+    with pytest.raises(ValueError, match="repetition_penalty"):
+        engine.generate([[1], [2]], [good, dict(good, repetition_penalty=-1)])
+    assert not engine.has_work()
