@@ -554,8 +554,6 @@ static long lg_lists(LogitsArgs& a, void* work, int sms) {
   a.bucket_shift = 8;  // (few tokens share a bucket, and with it a counter)
   while (((a.vocab - 1) >> a.bucket_shift) + 1 > LG_BUCKETS) ++a.bucket_shift;
   const int buckets = ((a.vocab - 1) >> a.bucket_shift) + 1;
-  const long listed = static_cast<long>(a.penal ? a.text + (a.cu != nullptr ? TREE_MAX : 0) : 0) + a.biases;
-  a.list_room = listed < a.vocab ? listed : a.vocab;
   char* at = static_cast<char*>(work);
   auto take = [&](long bytes) {
     char* was = at;
@@ -566,6 +564,9 @@ static long lg_lists(LogitsArgs& a, void* work, int sms) {
   a.lists = 1;
   while (a.lists < 8 && static_cast<long>(a.requests) * a.lists * 2 <= 2l * sms) a.lists *= 2;
   const long S = static_cast<long>(a.requests) * a.lists;
+  // (a list has each token once, and of the vocabulary only every lists-th)
+  const long listed = static_cast<long>(a.penal ? a.text + (a.cu != nullptr ? TREE_MAX : 0) : 0) + a.biases, most = (a.vocab + a.lists - 1) / a.lists;
+  a.list_room = listed < most ? listed : most;
   a.row_way = reinterpret_cast<uint4*>(take(a.cu != nullptr ? a.rows * 16l : 0));
   a.row_request = reinterpret_cast<int*>(take(a.cu != nullptr ? a.rows * 4l : 0));
   a.list_start = reinterpret_cast<int*>(take(S * (buckets + 1) * 4));

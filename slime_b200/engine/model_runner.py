@@ -1437,7 +1437,7 @@ class ModelRunner:
         if self.adjustments is None:
             if not req.sampling.adjusts:
                 return
-            self.adjustments = penalties.SlotAdjustments(self.max_batch, self.max_context, self.device)
+            self.adjustments = penalties.SlotAdjustments(self.max_batch, self.max_context, self.cfg.vocab_size, self.device)
         if self.adjustments.set(slot, req):
             if self.device.type == "cuda":
                 torch.cuda.current_stream().synchronize()

@@ -84,16 +84,25 @@ def _biases(samplings):
 class SlotAdjustments:
     """The same for decode slots, whose texts the host does not know up to the last token: the device keeps them, a step adds the token that it is fed."""
 
-    def __init__(self, slots: int, max_context: int, device):
+    def __init__(self, slots: int, max_context: int, vocab: int, device):
+        self.vocab = vocab
         self.text = torch.zeros(slots, max_context + 1, dtype=torch.int32, device=device)
         self.prompt_lens = torch.zeros(slots, dtype=torch.int32, device=device)
         self.numbers = torch.zeros(3, slots, device=device)
         self.numbers[0] = 1.0
         self.bias_ids = self.bias_values = None
         self.asked = [False] * slots
+        self._make_room()
+
+    def _make_room(self):
+        """The memory that every step works in, whatever the number of slots: captured steps, which run one after the other, would each keep their own."""
+        slots, width = self.text.shape
+        biases = 0 if self.bias_ids is None else self.bias_ids.shape[1]
+        size = max(ops.adjust_logits_workspace(n, self.vocab, self.text.device, text=width, biases=biases) for n in range(1, slots + 1))
+        self.work = torch.empty(size, dtype=torch.uint8, device=self.text.device) if size else None
 
     def set(self, slot: int, req) -> bool:
-        """The slot's next steps are of this request. True: the buffers of the biases are others now, and a captured step is stale."""
+        """The slot's next steps are of this request. True: the buffers of biases and workspace are others now, and a captured step is stale."""
         s = req.sampling
         if not (s.adjusts or self.asked[slot]):
             return False
@@ -112,6 +121,7 @@ class SlotAdjustments:
             if have:
                 grown[0][:, :have], grown[1][:, :have] = self.bias_ids, self.bias_values
             self.bias_ids, self.bias_values = grown
+            self._make_room()
         if self.bias_ids is not None:
             self.bias_ids[slot] = -1
             if need:
@@ -126,4 +136,5 @@ class SlotAdjustments:
         some = self.bias_ids is not None
         return ops.adjust_logits(
             logits, text, seq_lens, self.prompt_lens[:n], repetition=self.numbers[0, :n], frequency=self.numbers[1, :n], presence=self.numbers[2, :n],
-            bias_ids=self.bias_ids[:n] if some else None, bias_values=self.bias_values[:n] if some else None, out=logits)  # fmt: skip
+            bias_ids=self.bias_ids[:n] if some else None, bias_values=self.bias_values[:n] if some else None, out=logits,
+            workspace=self.work)  # fmt: skip

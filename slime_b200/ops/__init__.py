@@ -921,4 +921,4 @@ def router_gemm(x, w):
 
 # ---------------------------------------------------- drafted-token trees, logits before sampling
 from slime_b200.ops.tree import accept_tree, tree_attention  # noqa: E402, F401
-from slime_b200.ops.logits import adjust_logits  # noqa: E402, F401
+from slime_b200.ops.logits import adjust_logits, adjust_logits_workspace  # noqa: E402, F401

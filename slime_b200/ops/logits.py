@@ -23,13 +23,21 @@ def _workspace(rows: int, requests: int, vocab: int, text: int, biases: int, pen
     return size.value
 
 
+def adjust_logits_workspace(rows: int, vocab: int, device, *, requests: int | None = None, text: int = 0, biases: int = 0, penalties: bool = True,
+                            tree: bool = False) -> int:  # fmt: skip
+    """Bytes that ``adjust_logits`` works in for so many rows and tokens of a text (columns of ``tokens``) and biases of a request; 0: none."""
+    if torch.device(device).type != "cuda" or not (penalties or biases):
+        return 0
+    return _workspace(rows, rows if requests is None else requests, vocab, text if penalties else 0, biases, penalties, tree, _lib.sm_count(device))
+
+
 def _per_request(op: str, name: str, t, requests: int, device):
     if t is not None and (t.shape != (requests,) or t.dtype != torch.float32 or t.device != device or not t.is_contiguous()):
         raise ValueError(f"{op}: {name} must be {requests} contiguous fp32 values on {device}, not {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repetition=None, frequency=None, presence=None, bias_ids=None,
-                  bias_values=None, allowed=None, tree=None, out=None):  # fmt: skip
+                  bias_values=None, allowed=None, tree=None, out=None, workspace=None):  # fmt: skip
     """Logits [R, V] (bf16 or fp32, rows may be strided) as the requests want them sampled; ``out`` may be ``logits`` itself.
 
     ``tokens`` [S, L]: the text of each of S requests, of which the first ``lengths`` [S] count and the first ``prompt_lens`` [S] are prompt (None: none are).
@@ -43,6 +51,10 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     None: no such step; 1, 0 and 0 leave a request's logits as they are. ``tree`` = (drafted [R], parents [R], cu_nodes [S + 1]): row r belongs to a node of
     a tree of drafted tokens (``slime_b200.ops.tree``), and the drafted tokens of the node and those above it count as answered with. The root is the
     last token of the text already. Rows behind the last tree are left as they are. Without it row r is request r.
+
+    ``workspace``: bytes (uint8) for calls that run one after the other to share, at least as many as ``adjust_logits_workspace`` names. A captured call keeps the
+    memory that it works in for good, so a program that captures many gives them one. None: the call's own.
+
     Token ids, lengths and mask words are int32. Everything is worked out in fp32 and rounded once."""
     if logits.dim() != 2 or not (logits.dtype is _BF16 or logits.dtype is _F32):
         raise ValueError(f"adjust_logits: logits are [rows, vocabulary] in bf16 or fp32, not {tuple(logits.shape)} in {logits.dtype}")
@@ -69,6 +81,8 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
         fine = (allowed.shape == (R, -(-V // 32)) and allowed.dtype is _I32 and allowed.device == dev and (allowed.shape[1] <= 1 or allowed.stride(1) == 1))
     if not fine or tree is not None:
         _check(logits, tokens, lengths, prompt_lens, repetition, frequency, presence, bias_ids, bias_values, allowed, tree, out, S, penal)
+    if workspace is not None and not (workspace.dtype is torch.uint8 and workspace.device == dev and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0):
+        raise ValueError(f"adjust_logits: a workspace is uint8 on {dev}, in one piece from a boundary of 16 bytes, not {workspace.dtype} on {workspace.device}")
     if out is None:
         out = logits.new_empty(R, V)
     if _checks.enabled():
@@ -83,7 +97,7 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     if dev.index != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return adjust_logits(logits, tokens, lengths, prompt_lens, repetition=repetition, frequency=frequency, presence=presence, bias_ids=bias_ids,
-                                 bias_values=bias_values, allowed=allowed, tree=tree, out=out)  # fmt: skip
+                                 bias_values=bias_values, allowed=allowed, tree=tree, out=out, workspace=workspace)  # fmt: skip
     if V > 1 and logits.stride(1) != 1:
         logits = logits.contiguous()
     at = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
@@ -91,7 +105,12 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     text, pitch = (tokens.shape[1], tokens.stride(0)) if penal else (0, 0)
     sms = _tree._facts(dev)[0]
     size = _workspace(R, S, V, text, K, penal, tree is not None, sms) if penal or K else 0
-    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    if workspace is None:
+        work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    elif workspace.numel() < size:
+        raise ValueError(f"adjust_logits: a workspace of {workspace.numel()} bytes for a call that needs {size}")
+    else:
+        work = workspace
     rc = _lib.lib().sb_adjust_logits(
         _CALL(logits.data_ptr(), out.data_ptr(), at(tokens), at(lengths), at(prompt_lens), at(repetition), at(frequency), at(presence), at(bias_ids),
               at(bias_values), at(allowed), at(drafted), at(parents), at(cu_nodes), logits.stride(0), out.stride(0), pitch, K,

@@ -401,6 +401,36 @@ def test_logits_of_many_strided_rows_in_a_graph(dtype):
         assert torch.equal(cu, cu_then)
 
 
+def test_captured_logits_share_a_workspace():
+    """Two captured calls of other sizes, one replayed after the other, in memory that is full of something else; neither allocates any of its own. A smaller one is refused."""
+    from slime_b200 import ops
+
+    cases = [logits_case(R, V, L=L, K=K, parts=("repetition", "frequency", "presence", "bias")) for R, V, L, K in ((600, 4200, 70, 3), (130, 20011, 7000, 9))]
+    sizes = [ops.adjust_logits_workspace(*x.shape, "cuda", text=kw["tokens"].shape[1], biases=kw["bias_ids"].shape[1]) for x, kw, _ in cases]
+    assert min(sizes) > 0
+    work = torch.full((max(sizes),), 0x7F, dtype=torch.uint8, device="cuda")
+    held = []
+    for x, _, dev in cases:
+        y, out = x.cuda(), torch.empty(x.shape, device="cuda")
+        ops.adjust_logits(y, **dev, out=out, workspace=work)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.max_memory_allocated()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.adjust_logits(y, **dev, out=out, workspace=work)
+        assert torch.cuda.max_memory_allocated() - before < min(sizes)
+        held.append((graph, out, y))
+    want = [oracle.adjusted(x, **kw)[0] for x, kw, _ in cases]
+    for i in (0, 1, 1, 0):
+        held[i][1].fill_(5.0)
+        work.fill_(0x55)
+        held[i][0].replay()
+        same_logits(held[i][1], want[i], torch.float32, spread=7040)
+    with pytest.raises(ValueError, match="workspace"):
+        ops.adjust_logits(held[0][2], **cases[0][2], workspace=work[: sizes[0] - 16])
+
+
 # ------------------------------------------------------------------------------------------------------------- accept
 def accept_case(sizes, seed=0, share=0.8, holes=0.0):
     g = torch.Generator().manual_seed(seed)
@@ -597,3 +627,37 @@ def test_captured_decode_steps_adjust_their_logits():
         got.append([[r.output_ids for r in x] + [r.output_logprobs for r in x] for x in (first, plain, again)])
         e.shutdown()
     assert got[0] == got[1]
+
+
+@pytest.mark.parametrize("graphs", [False, True])
+def test_steps_of_many_requests_with_a_wide_context_adjust_their_logits(graphs):
+    """A context as wide as the engine's default, and more requests than the operator takes in one launch (a row of 512 tokens is one CTA's, 8 for each SM): a presence penalty lets no
+    token come twice, a negative frequency penalty no other than the first, biases none but a few, whatever was asked beside it; a request has a text of 9000 tokens."""
+    from slime_b200 import ops
+    from slime_b200.engine.engine import Engine
+    from slime_b200.engine.server_args import ServerArgs
+    from slime_b200.models.config import get_preset
+
+    n = 8 * torch.cuda.get_device_properties(0).multi_processor_count + 16
+    g = torch.Generator().manual_seed(1)
+    prompts = [torch.randint(0, 500, (3 + i % 5,), generator=g).tolist() for i in range(n)]
+    prompts[8] = torch.randint(0, 500, (9000,), generator=g).tolist()
+    few = {t: -1e9 for t in range(512) if t % 50 != 7}
+    asks = [dict(presence_penalty=1e6), dict(frequency_penalty=-1e6), dict(), dict(logit_bias=few)]
+    e = Engine(get_preset("tiny"), ServerArgs(page_size=16, max_running_requests=n, context_length=32768, disable_cuda_graph=not graphs),
+               device="cuda", num_pages=2 * n + 700)  # fmt: skip
+    e.weights.init_random(0, std=0.2)
+    reqs = e.generate(prompts, [dict(max_new_tokens=12 if i < n - 400 else 5, temperature=0, ignore_eos=True, **asks[i % 4]) for i in range(n)])
+    a = e.runner.adjustments
+    assert a.work.numel() == ops.adjust_logits_workspace(n, 512, "cuda", text=32769, biases=512) > 0
+    assert a.work.numel() <= n * (512 * 12 + 16) + 64  # (not by the width of the context)
+    for i, r in enumerate(reqs):
+        out = r.output_ids
+        assert len(out) == (12 if i < n - 400 else 5)
+        if i % 4 == 0:
+            assert len(set(out)) == len(out)
+        elif i % 4 == 1:
+            assert set(out) == {out[0]}
+        elif i % 4 == 3:
+            assert all(t % 50 == 7 for t in out)
+    e.shutdown()

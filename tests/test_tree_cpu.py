@@ -259,3 +259,28 @@ def test_accepted_rows_of_one_byte_elements(width):
     after = oracle.moved(caches, table, ctx, [w[0] for w in want], [w[2] for w in want], 4)
     ops.accept_tree(sampled, drafted, parents, cu, 9, k_caches=caches[0], block_table=table, context_lens=torch.tensor(ctx, dtype=torch.int32), page_size=4)
     assert torch.equal(caches[0], after[0])
+
+
+def test_workspace_of_adjusted_logits():
+    x, ids = torch.zeros(2, 5), torch.zeros(2, 3, dtype=torch.int32)
+    assert ops.adjust_logits_workspace(2, 5, "cpu", text=3) == 0
+    kw = dict(tokens=ids, lengths=ids[:, 0].contiguous(), frequency=torch.zeros(2))
+    assert torch.equal(ops.adjust_logits(x, **kw, workspace=torch.empty(0, dtype=torch.uint8)), x)
+    for bad in (torch.empty(64), torch.empty(64, dtype=torch.uint8)[::2], torch.empty(64, dtype=torch.uint8)[1:]):
+        with pytest.raises(ValueError, match="workspace"):
+            ops.adjust_logits(x, **kw, workspace=bad)
+
+
+@pytest.mark.parametrize("requests, lists", [(16, 8), (32, 8), (64, 4), (148, 2), (149, 1), (256, 1)])
+@pytest.mark.parametrize("biases", [0, 300])
+def test_workspace_is_no_larger_than_what_lists_of_distinct_tokens_can_hold(requests, lists, biases):
+    """With several lists of a request each has every second, fourth or eighth token of the vocabulary at most, however long the text may be."""
+    from slime_b200.ops import _lib, logits
+
+    if not _lib.available():
+        pytest.skip("the kernel library is not built")
+    vocab, text, sms = 151936, 32769, 148
+    size = logits._workspace(requests, requests, vocab, text, biases, True, False, sms)
+    most = min(text + biases, -(-vocab // lists))
+    starts = -(-vocab // 256) + 1
+    assert size <= requests * lists * (most * (12 if biases else 8) + starts * 4) + 64
