@@ -9,7 +9,7 @@
 // memory and puts in the listed ones while their lines are near. A request needs no table of the vocabulary's size that would have to be
 // kept, cleared and read, only its text. (Putting them in behind the whole copy cost 55 us of 195 at 763 rows of 151936: single
 // words to lines that had left the L2.) A small call takes one launch, `logits_kernel`, that keeps a chunk of a row in registers while it counts.
-// Biases of a token are added up in list order by one thread: nothing depends on an order of arrival. Logits that the mask hides are not read.
+// Biases of a token are added up in list order: nothing depends on an order of arrival. Logits that the mask hides are not read.
 // Everything is worked out in fp32 and rounded once. What bounds it: reading and writing the logits, 16 bytes a thread and access; a row that
 // does not start on such a boundary is cut at the boundaries all the same, and its two ends go element by element.
 // Measured (B200): 256 rows of 151936 fp32, texts of 1150: 64 us, of which the rows take 46 (6.8 TB/s) and counting, a chain of atomics and loads in few CTAs, the
@@ -120,8 +120,9 @@ __device__ __forceinline__ float lg_used(float v, bool seen, int times, float re
   return v + bias;
 }
 
-// What there is of a token: in the prompt, has a bias, was drafted, and how many times it was answered with. lg_text: each token of a request's text.
-enum : int { LG_PROMPT = 1 << 30, LG_BIAS = 1 << 29, LG_DRAFT = 1 << 28 };
+// What there is of a token: in the prompt, has a bias, was drafted, its bias is listed more than once, one of the bias's entries has been seen to; and how many
+// times it was answered with. lg_text: each token of a request's text.
+enum : int { LG_PROMPT = 1 << 30, LG_BIAS = 1 << 29, LG_DRAFT = 1 << 28, LG_TWICE = 1 << 27, LG_TAKEN = 1 << 26, LG_TIMES = LG_TAKEN - 1 };
 constexpr int LG_FLY = 4;  // tokens whose reads are under way together
 template <typename F>
 __device__ __forceinline__ void lg_text(const LogitsArgs& a, int req, int threads, const F& each) {
@@ -135,6 +136,35 @@ __device__ __forceinline__ void lg_text(const LogitsArgs& a, int req, int thread
       if (static_cast<unsigned>(t[x]) >= static_cast<unsigned>(a.vocab)) t[x] = -1;
     }
     each(i0, t);
+  }
+}
+
+// Biases of a request, once all entries are marked (lg_mark): `each` gets every token with a place, once, and its bias. The first entry of a token to come stands for it;
+// where there are more of them a warp goes through the list for that token and adds up in the list's order.
+__device__ __forceinline__ void lg_mark(int* at) {
+  if (atomicOr(at, LG_BIAS) & LG_BIAS) atomicOr(at, LG_TWICE);
+}
+template <typename Place, typename F>
+__device__ __forceinline__ void lg_biases(const int* ids, const float* values, int K, int threads, const Place& place, const F& each) {
+  const int lane = threadIdx.x & 31;
+  for (int i0 = threadIdx.x - lane; i0 < K; i0 += threads) {
+    const int i = i0 + lane, id = i < K ? ids[i] : -1;
+    int* at = place(id);
+    const int what = at != nullptr ? atomicOr(at, LG_TAKEN) : LG_TAKEN;
+    const bool first = (what & LG_TAKEN) == 0;
+    float bias = first ? values[i] : 0.f;
+    for (uint32_t more = __ballot_sync(0xffffffffu, first && (what & LG_TWICE)); more != 0; more &= more - 1) {
+      const int src = __ffs(more) - 1, t = __shfl_sync(0xffffffffu, id, src);
+      float sum = 0.f;
+      for (int j0 = 0; j0 < K; j0 += 32) {
+        const int j = j0 + lane;
+        const bool same = j < K && ids[j] == t;
+        const float v = same ? values[j] : 0.f;
+        for (uint32_t hit = __ballot_sync(0xffffffffu, same); hit != 0; hit &= hit - 1) sum += __shfl_sync(0xffffffffu, v, __ffs(hit) - 1);
+      }
+      if (lane == src) bias = sum;
+    }
+    if (first) each(id, at, what, bias);
   }
 }
 
@@ -209,28 +239,19 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
       }
     }
   }
-  int any_bias = 0, again = 0;
+  int any_bias = 0;
   const int K = a.biases;
   const int* ids = a.bias_ids + req * a.bias_row;
   const float* values = a.bias_values + req * a.bias_row;
   for (int i = tid; i < K; i += LG_THREADS)
     if (const int at = place(ids[i]); at >= 0) {
-      again |= (atomicOr(&count[at], LG_BIAS) & LG_BIAS) != 0;  // listed twice
+      lg_mark(&count[at]);
       any_bias = 1;
     }
-  again = __syncthreads_or(again);
   any_bias = __syncthreads_or(any_bias);
   if (any_bias) {
-    for (int i = tid; i < K; i += LG_THREADS)
-      if (const int id = ids[i], at = place(id); at >= 0) {
-        float sum = values[i];
-        if (again) {  // all entries of a token add up the same: which one is written does not matter
-          sum = 0.f;
-          for (int j = 0; j < K; ++j)
-            if (ids[j] == id) sum += values[j];
-        }
-        bias[at] = sum;
-      }
+    lg_biases(ids, values, K, LG_THREADS, [&](int t) { const int at = place(t); return at >= 0 ? &count[at] : nullptr; },
+              [&](int, int* at, int, float sum) { bias[at - count] = sum; });
     __syncthreads();
   }
   // ---- the row
@@ -248,7 +269,7 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
       for (int k = 0; k < 4; ++k) {
         const int c = cs[k];
         float v = static_cast<float>(e[q + k]);
-        if (c != 0) v = lg_used(v, (c & ~LG_BIAS) != 0, c & (LG_DRAFT - 1), rep, freq, pres, any_bias ? bias[at + q + k] : 0.f);
+        if (c != 0) v = lg_used(v, (c & (LG_PROMPT | LG_TIMES)) != 0, c & LG_TIMES, rep, freq, pres, any_bias ? bias[at + q + k] : 0.f);
         if ((shown >> (q + k) & 1) == 0) v = -INFINITY;
         e[q + k] = static_cast<T>(v);
       }
@@ -390,17 +411,9 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
           if (came) brought_x = 1;
         }
     }
-    // biases: the first of a token's entries to come lists the token. again: a token is listed twice. mine: entries, one bit each
-    const bool marks = K <= 32 * THREADS;
-    uint32_t mine = 0;
-    int again = 0;
-    for (int i = tid, x = 0; i < K; i += THREADS, ++x)
-      if (int* at = place(ids[i], came); at != nullptr) {
-        const bool leads = (atomicOr(at, LG_BIAS) & LG_BIAS) == 0;
-        if (leads && marks) mine |= 1u << x;
-        again |= !leads;
-      }
-    again = __syncthreads_or(again);
+    for (int i = tid; i < K; i += THREADS)
+      if (int* at = place(ids[i], came); at != nullptr) lg_mark(at);
+    __syncthreads();
     // ---- by bucket: how many there are, where each bucket begins, then the tokens (in any order within a bucket)
     if (direct) {
       for (int at = tid; at < 2 * HASH; at += THREADS)
@@ -458,22 +471,7 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
       if (brought_x)
         if (const int what = *place(tree_t[tid], came); (what & LG_BIAS) == 0) put(tree_t[tid], what, 0.f);
     }
-    for (int i = tid, x = 0; i < K; i += THREADS, ++x) {
-      const int id = ids[i];
-      if (marks && (mine >> x & 1) == 0) continue;
-      const int* at = place(id, came);
-      if (at == nullptr) continue;
-      bool leads = true;
-      for (int j = 0; !marks && leads && j < i; ++j) leads = ids[j] != id;
-      if (!leads) continue;
-      float bias = values[i];
-      if (again) {
-        bias = 0.f;
-        for (int j = 0; j < K; ++j)
-          if (ids[j] == id) bias += values[j];
-      }
-      put(id, *at, bias);
-    }
+    lg_biases(ids, values, K, THREADS, [&](int t) { return place(t, came); }, [&](int t, int*, int what, float bias) { put(t, what, bias); });
     if (pass + 1 < passes) __syncthreads();
   }
   pdl_launch_dependents();  // not before: rows that wait for the lists would slow the counting down (a tenth of the call at 256 rows of 151936)
@@ -535,7 +533,7 @@ logits_row_kernel(const __grid_constant__ LogitsArgs a) {
     const int t = entry.x, what = entry.y;
     if (t < lo || t >= hi) continue;
     if (a.allowed != nullptr && (a.allowed[r * a.allowed_row + (t >> 5)] >> (t & 31) & 1) == 0) continue;  // (hidden: -infinity already)
-    int times = what & (LG_DRAFT - 1);
+    int times = what & LG_TIMES;
     if (what & LG_DRAFT) {  // drafted nodes of this token on the way to this row
       const uint4 way = a.row_way[r];
       const int first = a.cu[req], n = min(min(a.cu[req + 1], a.rows) - first, TREE_MAX);

@@ -12,6 +12,7 @@ from slime_b200.ops import _checks, _lib, reference, tree as _tree
 
 _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 MAX_VOCAB = 1 << 25  # the kernels sort tokens into 1024 buckets, each of which is within a table of 32768 tokens
+MAX_TEXT = (1 << 26) - 256  # a token is counted in 26 bits, drafted nodes included
 _CALL = struct.Struct("28q").pack  # arguments of the C entry
 
 
@@ -66,7 +67,7 @@ def adjust_logits(logits, tokens=None, lengths=None, prompt_lens=None, *, repeti
     # (as in ``tree.tree_attention``: one expression for what is in order)
     fine = V <= MAX_VOCAB and (out is None or (out.shape == logits.shape and out.dtype is dtype and out.device == dev and (V <= 1 or out.stride(1) == 1)))
     if fine and penal:
-        fine = (tokens is not None and lengths is not None and tokens.dim() == 2 and tokens.shape[0] == S and tokens.dtype is _I32 and tokens.device == dev
+        fine = (tokens is not None and lengths is not None and tokens.dim() == 2 and tokens.shape[0] == S and tokens.shape[1] <= MAX_TEXT and tokens.dtype is _I32 and tokens.device == dev
                 and (tokens.shape[1] <= 1 or tokens.stride(1) == 1) and lengths.shape == (S,) and lengths.dtype is _I32 and lengths.device == dev
                 and lengths.is_contiguous())  # fmt: skip
         if prompt_lens is not None:
@@ -134,6 +135,8 @@ def _check(logits, tokens, lengths, prompt_lens, repetition, frequency, presence
             raise ValueError(f"{op}: penalties need the tokens of the requests and their lengths")
         _tree._shape(op, "tokens", tokens, S, None)
         _tree._shape(op, "lengths", lengths, S)
+        if tokens.shape[1] > MAX_TEXT:
+            raise ValueError(f"{op}: texts of at most {MAX_TEXT} tokens, not {tokens.shape[1]}")
         if tokens.dtype != _I32 or tokens.device != dev or (tokens.shape[1] > 1 and tokens.stride(1) != 1):
             raise ValueError(f"{op}: tokens must be int32 rows on {dev}")
         _tree._ints(op, dev, lengths=lengths)

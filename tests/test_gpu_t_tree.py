@@ -431,6 +431,57 @@ def test_captured_logits_share_a_workspace():
         ops.adjust_logits(held[0][2], **cases[0][2], workspace=work[: sizes[0] - 16])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R", [2, 125])  # one launch, two
+@pytest.mark.parametrize("K", [37, 2999, 20011])
+@pytest.mark.parametrize("what", ["distinct", "one twice", "all twice", "all the same", "last place"])
+def test_logits_of_long_lists_of_biases(dtype, R, K, what):
+    """Whole numbers as biases, so that sums of them are exact; beside penalties of a text that shares tokens with the list."""
+    from slime_b200 import ops
+
+    V = 20011
+    x, kw, _ = logits_case(R, V, L=50, K=K, dtype=dtype, parts=("repetition", "frequency", "bias"))
+    g = torch.Generator().manual_seed(K)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(R)]).int()
+    if what == "one twice":
+        ids[:, K // 2] = ids[:, 1]
+    elif what == "all twice":
+        ids[:, K // 2 :] = ids[:, : K - K // 2].flip(1)
+    elif what == "all the same":
+        ids[:] = V - 1
+    elif what == "last place":
+        ids[:, -1] = ids[:, 0]
+    kw["bias_ids"], kw["bias_values"] = ids, torch.randint(-8, 9, (R, K), generator=g).float()
+    kw["tokens"][:, ::2] = ids[:, : 1].expand(-1, 25)
+    dev = {n: v.cuda() for n, v in kw.items()}
+    y = x.cuda()
+    want, _ = oracle.adjusted(x, **kw)
+    got = ops.adjust_logits(y, **dev)
+    same_logits(got, want, dtype, spread=90 + float(kw["bias_values"].sum(1).abs().max()))
+    for _ in range(2):
+        assert torch.equal(got.nan_to_num(9.0), ops.adjust_logits(y, **dev).nan_to_num(9.0))
+
+
+def test_a_token_listed_twice_does_not_cost_every_entry_a_look_at_the_list():
+    from slime_b200 import ops
+
+    x = torch.randn(64, 151936, device="cuda")
+    ids = (7 * torch.arange(12000, dtype=torch.int32, device="cuda")).repeat(64, 1)
+    twice, values = ids.clone(), torch.ones(64, 12000, device="cuda")
+    twice[:, 5000] = twice[:, 3]
+
+    def best(i):
+        ends = [(torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)) for _ in range(8)]
+        for a, b in ends:
+            a.record()
+            ops.adjust_logits(x, bias_ids=i, bias_values=values, out=x)
+            b.record()
+        torch.cuda.synchronize()
+        return min(a.elapsed_time(b) for a, b in ends)
+
+    assert best(twice) < 5 * best(ids)  # (once 100 times as much)
+
+
 # ------------------------------------------------------------------------------------------------------------- accept
 def accept_case(sizes, seed=0, share=0.8, holes=0.0):
     g = torch.Generator().manual_seed(seed)

@@ -284,3 +284,9 @@ def test_workspace_is_no_larger_than_what_lists_of_distinct_tokens_can_hold(requ
     most = min(text + biases, -(-vocab // lists))
     starts = -(-vocab // 256) + 1
     assert size <= requests * lists * (most * (12 if biases else 8) + starts * 4) + 64
+
+
+def test_texts_that_could_not_be_counted_are_refused():
+    wide = torch.zeros(2, 1, dtype=torch.int32).expand(2, 1 << 26)
+    with pytest.raises(ValueError, match="texts of at most"):
+        ops.adjust_logits(torch.zeros(2, 5), tokens=wide, lengths=torch.zeros(2, dtype=torch.int32), presence=torch.ones(2))
