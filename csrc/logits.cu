@@ -197,7 +197,7 @@ logits_kernel(const __grid_constant__ LogitsArgs a) {
     req = found;
     if (req < 0) return;  // behind the last tree: left as it is
     first = a.cu[req];
-    n = min(min(a.cu[req + 1], a.rows) - first, TREE_MAX);
+    n = first < 0 ? 0 : min(min(a.cu[req + 1], a.rows) - first, TREE_MAX);
   }
   const float rep = a.repetition != nullptr ? a.repetition[req] : 1.f;
   const float freq = a.frequency != nullptr ? a.frequency[req] : 0.f;
@@ -321,8 +321,8 @@ logits_count_kernel(const __grid_constant__ LogitsArgs a) {
     tree_t[i] = a.drafted[first + i];
   }
   __syncthreads();
-  if (first >= 0 && part == 0)
-    for (int r = first + tid; r < until; r += THREADS) {  // rows of the tree: whose they are, and the nodes on the way to them (the root is the text's last token)
+  if (a.cu != nullptr && part == 0)
+    for (int r = max(first, 0) + tid; r < until; r += THREADS) {  // rows of the tree: whose they are, and the nodes on the way to them (the root is the text's last token)
       uint32_t set[4] = {0, 0, 0, 0};
       if (r - first < n) tree_way_up([&](int j) { return tree_p[j]; }, r - first, set);
       a.row_way[r] = make_uint4(set[0] & ~1u, set[1], set[2], set[3]);

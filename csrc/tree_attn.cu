@@ -28,6 +28,7 @@ tree_attn_kernel(const T* __restrict__ q, const T* __restrict__ k_cache, const T
   const int t = blockIdx.x, h = blockIdx.y * 4 + warp;
   if (h >= Hq || t < cu[0] || t >= cu[B]) return;
   const int b = tree_of_row(cu, B, t);
+  if (cu[b] < 0) return;
   const int i = t - cu[b], n = min(cu[b + 1] - cu[b], max_nodes);
   if (i >= n) return;
   const int kvh = h / (Hq / Hkv);

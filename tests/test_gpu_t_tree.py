@@ -566,6 +566,30 @@ def test_acceptance_of_one_byte_caches(dtype, H, D, left):
             assert torch.equal(dev.cpu(), after)
 
 
+@pytest.mark.parametrize("heads", [(14, 2, 64), (4, 2, 8)])
+@pytest.mark.parametrize("copies", [1, 300])  # logits in one launch, in two
+def test_a_tree_that_begins_in_front_of_the_rows_is_none(heads, copies):
+    """A first number below zero: nothing in front of the packed rows is read, and the other trees are what they are. (Checks of indices refuse such a call.)"""
+    from slime_b200 import ops
+
+    sizes, ctx = [2] + [4, 1] * copies, [9] + [5, 30] * copies
+    q, k, v, table, c, cu, parents = attention_case(sizes, ctx, heads, 16, seed=2)
+    bad = cu.clone()
+    bad[0] = -3
+    want = ops.tree_attention(q, k, v, table, c, cu, parents, 16, 4)
+    got = ops.tree_attention(q, k, v, table, c, bad, parents, 16, 4, out=torch.full_like(q, 7.0))
+    assert torch.equal(got[2:], want[2:]) and (got[:2] == 7).all()
+    x, _, dev = logits_case(len(sizes), 4100, sizes, L=40)
+    drafted = dev["tree"][0]
+    want = ops.adjust_logits(x.cuda(), **{**dev, "tree": (drafted, parents, cu)})
+    got = ops.adjust_logits(x.cuda(), **{**dev, "tree": (drafted, parents, bad)})
+    assert torch.equal(got[2:].nan_to_num(9.0), want[2:].nan_to_num(9.0))
+    sampled = drafted.roll(-1)
+    want = ops.accept_tree(sampled, drafted, parents, cu, 4)
+    got = ops.accept_tree(sampled, drafted, parents, bad, 4)
+    assert all(torch.equal(a[1:], b[1:]) for a, b in zip(got, want)) and int(got[2][0]) == 0
+
+
 # ------------------------------------------------------------------------------------------------------- a whole round
 def test_a_round_of_drafted_trees_is_ordinary_decoding():
     """One attention layer with a vocabulary behind it, in fp32 (close calls of the sampler aside, both forms then draw the same tokens): two rounds of trees, penalties included,
