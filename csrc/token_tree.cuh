@@ -9,6 +9,7 @@
 namespace sb {
 
 constexpr int TREE_MAX = 128;  // nodes of a tree
+constexpr long TREE_MAX_KEYS = 0x7fffff00l;  // keys that a request can have: nodes behind them, and the rest of their tile, stay within an int
 
 // Tree of packed row t: the largest b with cu[b] <= t, given cu[0] <= t < cu[B].
 __device__ __forceinline__ int tree_of_row(const int* __restrict__ cu, int B, int t) {

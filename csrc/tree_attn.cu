@@ -103,7 +103,7 @@ extern "C" int sb_tree_attn(const void* q, const void* k_cache, const void* v_ca
   if (rows <= 0 || B <= 0 || Hq <= 0) return 0;
   if (D > sb::TA_MAXD || D <= 0) return -1;
   if (Hkv <= 0 || Hq % Hkv != 0 || page_size <= 0 || max_nodes <= 0 || max_nodes > sb::TREE_MAX || max_pages < 0 ||
-      static_cast<long>(max_pages) * page_size > 0x7fffffffl)
+      static_cast<long>(max_pages) * page_size > sb::TREE_MAX_KEYS)
     return (int)cudaErrorInvalidValue;
   const dim3 grid(rows, (Hq + 3) / 4), block(128);
   if (f32)

@@ -911,7 +911,7 @@ struct TtPlan {
 };
 // tokens: most keys a request can have. false where the kernel does not cover the call.
 static bool tree_attn_plan(int B, int Hq, int Hkv, int D, int max_nodes, long tokens, int whole, int sms, TtPlan& p) {
-  if (B <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq / Hkv > 128 || (D != 64 && D != 128) || max_nodes <= 0 || max_nodes > TREE_MAX || tokens <= 0 || tokens > 0x7fffffffl) return false;
+  if (B <= 0 || Hkv <= 0 || Hq % Hkv != 0 || Hq / Hkv > 128 || (D != 64 && D != 128) || max_nodes <= 0 || max_nodes > TREE_MAX || tokens <= 0 || tokens > TREE_MAX_KEYS) return false;
   const int G = Hq / Hkv, rows = max_nodes * G;
   p.tiles = max_nodes > 128 / G ? 2 : 1;
   p.copies = rows <= 32 ? 4 : (rows <= 64 ? 2 : 1);

@@ -290,3 +290,18 @@ def test_texts_that_could_not_be_counted_are_refused():
     wide = torch.zeros(2, 1, dtype=torch.int32).expand(2, 1 << 26)
     with pytest.raises(ValueError, match="texts of at most"):
         ops.adjust_logits(torch.zeros(2, 5), tokens=wide, lengths=torch.zeros(2, dtype=torch.int32), presence=torch.ones(2))
+
+
+def test_page_tables_whose_last_nodes_would_pass_32_bits_are_refused():
+    """A context that fills a table of 2^31 tokens has no place for nodes that an int can count; both entries of tree attention refuse the table before a launch."""
+    import ctypes
+
+    from slime_b200.ops import _lib
+
+    if not _lib.available():
+        pytest.skip("the kernel library is not built")
+    lib, size = _lib.lib(), ctypes.c_long()
+    for tokens, fits in (((1 << 31) - 256, True), ((1 << 31) - 128, False), ((1 << 31) - 1, False), (1 << 31, False)):
+        assert (lib.sb_tree_attn_plan(1, 2, 2, 64, 4, tokens, 0, 148, ctypes.byref(size)) == 0) == fits
+        if not fits:
+            assert lib.sb_tree_attn(*[None] * 9, 4, 1, 2, 2, 64, 1, min(tokens, (1 << 31) - 1), 100, 4, *[0] * 7, 1.0, 0, None) == 1
