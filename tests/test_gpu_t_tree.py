@@ -131,6 +131,28 @@ def test_attention_beside_numbers_that_are_not_finite(heads, sizes, ctx, what):
     assert rows.any() and ((got - want).abs() <= bound(want, mass, torch.bfloat16, heads[2]))[rows].all()
 
 
+@pytest.mark.parametrize("heads", [(8, 2, 64), (16, 4, 128), (6, 2, 40)])
+def test_attention_of_caches_laid_out_otherwise(heads):
+    """Heads outside slots, one head for all, a head of its own whose pitch means nothing, keys and values of other pitches, queries with heads outside rows."""
+    from slime_b200 import ops
+
+    Hq, Hkv, D = heads
+    q, k, v, table, c, cu, parents = attention_case([9, 1, 33], [300, 17, 65], heads, 16)
+    rest = (table, c, cu, parents, 16, 33)
+    turned = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    want = ops.tree_attention(q, k, v, *rest)
+    assert torch.equal(want, ops.tree_attention(turned(q), turned(k), v, *rest))
+    assert torch.equal(want, ops.tree_attention(q, torch.cat([k, k], 1)[:, :Hkv], turned(v), *rest))
+    one = [x[:, :1].contiguous() for x in (k, v)]
+    same = ops.tree_attention(q, *(x.repeat(1, Hkv, 1) for x in one), *rest)
+    assert torch.equal(same, ops.tree_attention(q, *(x.expand(-1, Hkv, -1) for x in one), *rest))
+    lone = ops.tree_attention(q, *one, *rest)
+    odd = [x.as_strided(x.shape, (D, 3, 1)) for x in one]  # (the pitch of a single head)
+    want, mass = oracle.attention(q, *one, table, c, cu, parents, 16, D**-0.5)
+    for got in (lone, ops.tree_attention(q, *odd, *rest)):
+        assert ((got.double().cpu() - want).abs() <= bound(want, mass, torch.bfloat16, D)).all()
+
+
 @pytest.mark.parametrize("shape", ["chain", "star"])
 def test_attention_of_chains_and_stars(shape):
     from slime_b200 import ops
@@ -735,4 +757,70 @@ def test_steps_of_many_requests_with_a_wide_context_adjust_their_logits(graphs):
             assert set(out) == {out[0]}
         elif i % 4 == 3:
             assert all(t % 50 == 7 for t in out)
+    e.shutdown()
+
+
+@pytest.mark.parametrize("vocab, requests", [(512, 3), (20011, 40)])  # one launch, two
+def test_chains_of_guesses_are_adjusted_in_place(vocab, requests):
+    """The form that a speculating engine calls: rows for the last token of a text and the guesses behind it, in place, among requests that ask for nothing and rows that belong to none."""
+    from slime_b200.engine import penalties
+    from slime_b200.engine.request import Request, SamplingParams
+
+    g = torch.Generator().manual_seed(vocab)
+    ints = lambda n, hi=vocab: torch.randint(0, hi, (n,), generator=g).tolist()  # noqa: E731
+    asks = [dict(repetition_penalty=1.3, frequency_penalty=0.4), dict(), dict(presence_penalty=0.7, logit_bias={3: 2.0, 9: -1.5, 10**6: 4.0}),
+            dict(frequency_penalty=-0.2, presence_penalty=0.1, repetition_penalty=0.8)]  # fmt: skip
+    reqs, ids, sizes = [], [], []
+    for i in range(requests):
+        r = Request(rid=str(i), input_ids=ints(4 + 31 * i, 60), sampling=SamplingParams(**asks[i % 4]))
+        r.output_ids = ints(1 + 7 * i, 60)
+        reqs.append(r)
+        sizes.append(1 + i % 5)
+        ids += [r.output_ids[-1]] + ints(sizes[-1] - 1, 60)
+    spare = 2
+    cu = torch.tensor([0] + sizes).cumsum(0).int()
+    ids += [5] * spare
+    x = 3 * torch.randn(len(ids), vocab, generator=g)
+    logits = x.cuda()
+    assert penalties.adjust(logits, reqs, (torch.tensor(ids, dtype=torch.int32, device="cuda"), cu.cuda())) is logits
+    got = logits.cpu().double()
+    for i, r in enumerate(reqs):
+        s, a = r.sampling, int(cu[i])
+        for d in range(sizes[i]):
+            text, n = r.all_ids() + ids[a + 1 : a + 1 + d], len(r.input_ids)
+            f = lambda v: torch.tensor([v])  # noqa: E731
+            bias = {t: v for t, v in (s.logit_bias or {}).items()}
+            want, _ = oracle.adjusted(x[a + d : a + d + 1], torch.tensor([text]), torch.tensor([len(text)]), torch.tensor([n]), f(s.repetition_penalty),
+                                      f(s.frequency_penalty), f(s.presence_penalty), torch.tensor([list(bias)]) if bias else None,
+                                      torch.tensor([list(bias.values())]) if bias else None)  # fmt: skip
+            # five roundings of fp32 of values below 40 + 0.4 times the text's length, and penalties that are themselves rounded
+            torch.testing.assert_close(got[a + d : a + d + 1], want, rtol=9 * F32, atol=10 * F32 * (40 + len(text)))
+            if not s.adjusts:
+                assert torch.equal(logits[a + d].cpu(), x[a + d])
+    assert torch.equal(logits[-spare:].cpu(), x[-spare:])
+
+
+def test_speculating_requests_keep_their_penalties():
+    from slime_b200.engine.engine import Engine
+    from slime_b200.engine.server_args import ServerArgs
+    from slime_b200.models.config import ModelConfig
+
+    cfg = ModelConfig(num_layers=2, hidden_size=128, num_attention_heads=4, num_query_groups=2, kv_channels=64, ffn_hidden_size=256, vocab_size=512, rotary_base=1e4,
+                      tie_word_embeddings=False, mtp_num_layers=1, qk_layernorm=True, model_arch="Qwen3ForCausalLM")  # fmt: skip
+    e = Engine(cfg, ServerArgs(page_size=16, max_running_requests=8, context_length=512, speculative_algorithm="EAGLE", speculative_num_steps=3,
+                               speculative_num_draft_tokens=4), device="cuda", num_pages=400)  # fmt: skip
+    e.weights.init_random(0, std=0.2)
+    few = {t: -1e9 for t in range(512) if t % 50 != 7}
+    asks = [dict(presence_penalty=1e6), dict(frequency_penalty=-1e6), dict(), dict(logit_bias=few)]
+    prompts = [[(5 * i + 3 * j) % 500 for j in range(6 + i)] for i in range(8)]
+    for temperature in (0, 1.0):
+        reqs = e.generate(prompts, [dict(max_new_tokens=30, temperature=temperature, ignore_eos=True, **asks[i % 4]) for i in range(8)])
+        for i, r in enumerate(reqs):
+            assert len(r.output_ids) == 30
+            if i % 4 == 0:
+                assert len(set(r.output_ids)) == 30
+            elif i % 4 == 1:
+                assert len(set(r.output_ids)) == 1
+            elif i % 4 == 3:
+                assert all(t % 50 == 7 for t in r.output_ids)
     e.shutdown()
