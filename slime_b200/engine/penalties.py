@@ -50,7 +50,7 @@ def adjust(logits, reqs, chains=None):
     for row, text in zip(tokens, texts):
         row[: len(text)] = torch.tensor(text, dtype=torch.int32)
     numbers = torch.tensor([_numbers(r.sampling) for r in reqs], dtype=torch.float32).t().contiguous().to(dev)
-    ids, values = _biases([r.sampling for r in reqs])
+    ids, values = _biases([r.sampling for r in reqs], logits.shape[1])
     tree = None
     if chains is not None:
         drafted, cu = chains
@@ -67,17 +67,17 @@ def _numbers(s):
     return s.repetition_penalty, s.frequency_penalty, s.presence_penalty
 
 
-def _biases(samplings):
-    """([B, K] token ids, -1 behind the last; [B, K] values), or (None, None)."""
-    K = max(len(s.logit_bias or ()) for s in samplings)
+def _biases(samplings, vocab: int):
+    """([B, K] token ids, -1 behind the last; [B, K] values), or (None, None). Tokens outside the vocabulary count for nothing and are left out."""
+    lists = [[(t, v) for t, v in (s.logit_bias or {}).items() if t < vocab] for s in samplings]
+    K = max(len(x) for x in lists)
     if K == 0:
         return None, None
-    ids, values = torch.full((len(samplings), K), -1, dtype=torch.int32), torch.zeros(len(samplings), K)
-    for b, s in enumerate(samplings):
-        if s.logit_bias:
-            n = len(s.logit_bias)
-            ids[b, :n] = torch.tensor(list(s.logit_bias), dtype=torch.int32)
-            values[b, :n] = torch.tensor(list(s.logit_bias.values()), dtype=torch.float32)
+    ids, values = torch.full((len(lists), K), -1, dtype=torch.int32), torch.zeros(len(lists), K)
+    for b, x in enumerate(lists):
+        if x:
+            ids[b, : len(x)] = torch.tensor([t for t, _ in x], dtype=torch.int32)
+            values[b, : len(x)] = torch.tensor([v for _, v in x], dtype=torch.float32)
     return ids, values
 
 
@@ -113,10 +113,10 @@ class SlotAdjustments:
             ids = torch.tensor(req.all_ids(), dtype=torch.int32)
             self.text[slot, : len(ids)] = ids.to(dev)
             self.prompt_lens[slot] = len(req.input_ids)
-        ids, values = _biases([s])
+        ids, values = _biases([s], self.vocab)
         need, have = 0 if ids is None else ids.shape[1], 0 if self.bias_ids is None else self.bias_ids.shape[1]
         if need > have:
-            room = max(16, 1 << (need - 1).bit_length())
+            room = min(max(16, 1 << (need - 1).bit_length()), self.vocab)
             grown = (torch.full((self.text.shape[0], room), -1, dtype=torch.int32, device=dev), torch.zeros(self.text.shape[0], room, device=dev))
             if have:
                 grown[0][:, :have], grown[1][:, :have] = self.bias_ids, self.bias_values

@@ -148,3 +148,19 @@ def test_a_refused_penalty_is_a_client_error_and_nothing_of_its_body_is_queued()
     with pytest.raises(ValueError, match="repetition_penalty"):
         engine.generate([[1], [2]], [good, dict(good, repetition_penalty=-1)])
     assert not engine.has_work()
+
+
+def test_biases_of_tokens_outside_the_vocabulary_take_no_room():
+    """They count for nothing, so a request that lists many of them leaves every slot's room for biases where it was, and no list is longer than the vocabulary."""
+    _, _, plain, _ = _pair("dense")
+    V = plain.cfg.vocab_size
+    junk = {V + i: 1.0 for i in range(5000)}
+    base = dict(max_new_tokens=4, ignore_eos=True, temperature=0)
+    prompts = _prompts(plain.cfg, 2)
+    want = plain.generate(prompts, [dict(base, logit_bias={3: 2.0, 5: -1.0}), dict(base)])
+    room = plain.runner.adjustments.bias_ids.shape[1]
+    got = plain.generate(prompts, [dict(base, logit_bias={**junk, 3: 2.0, 5: -1.0}), dict(base, logit_bias=junk)])
+    assert [r.output_ids for r in got] == [r.output_ids for r in want]
+    assert plain.runner.adjustments.bias_ids.shape[1] == room
+    plain.generate(prompts, dict(base, logit_bias={t: 0.5 for t in range(V)}))
+    assert plain.runner.adjustments.bias_ids.shape[1] <= V
