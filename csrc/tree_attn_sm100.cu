@@ -23,15 +23,20 @@
 // second launch joins the parts in order: the same bits on every run. With `whole` each CTA takes one item, so that a row's arithmetic does
 // not depend on the batch.
 //
-// Key and value tiles have a ring of buffers each, with a producer of its own, and the rings run on from one piece of work to the next. Every
-// waiter sees every phase of a barrier: a wait by parity cannot tell one phase from the next but one. Even rings give that to the groups, which
-// take tiles in turn; a ring of three buffers has six barriers for it. The scores of hidden nodes become -infinity by a bit mask per row, looked at in the last tiles only. Cache rows behind
-// the last node may hold anything: pages behind it are fetched from outside the cache, which reads as zero, and the rest of its page is
-// cleared in shared memory before the product of weights (zero) and values. So are nodes' values that are not finite: rows that see
-// such a node become NaN, and the others stay what they are.
-// Measured (B200, both launches, page size 16): 64 trees of 16 nodes over 3,000 tokens, 32 / 8 heads of 128: 149 us, 0.85 of the copy rate; 4 trees of 64 nodes over 28,000, 32 / 4
-// heads of 128: 135 us, 870 TFLOP/s, tensor pipe and special functions 45 % each; 256 trees of 3 to 9 nodes over 770, 14 / 2 heads of 64: 43 us, 0.37 of
-// the copy rate, bound by what lies between pieces of work (4000 cycles for a piece's 9000); one tree of 8 nodes over 1,000: 11 us.
+// Key and value tiles have a ring of buffers each, with a producer of its own, and the rings run on from one piece of work to the next. A wait by parity cannot tell
+// one phase of a barrier from the next but one, so every waiter sees every phase or knows that the ones before it are over. Even rings give that to the groups, which
+// take tiles in turn; a ring of three buffers has six barriers for it. Where pieces with one and with two query tiles follow each other, a buffer's last tile may have
+// been the other group's alone: then the queries of a piece, which come once both groups' scores of the piece before are done, and the accumulators, which are
+// read once its products are, stand for it.
+//
+// The scores of hidden nodes become -infinity by a bit mask per row, looked at in the last tiles only. Cache rows behind the last node may hold anything: pages
+// behind it are fetched from outside the cache, which reads as zero, and the rest of its page is cleared in shared memory before the product of weights (zero) and
+// values. So are nodes' values that are not finite: rows that see such a node become NaN, and the others stay what they are.
+//
+// Measured (B200, both launches, page size 16, bursts of a few ms at 1965 MHz): 64 trees of 16 nodes over 3,000 tokens, 32 / 8 heads of 128: 151 us, 0.83 of the copy
+// rate; 4 trees of 64 nodes over 28,000, 32 / 4 heads of 128: 139 us, 850 TFLOP/s, tensor pipe and special functions 45 % each (172 and 161 us in calls without a
+// pause, where the power cap holds the clock near 1500 MHz); 256 trees of 3 to 9 nodes over 770, 14 / 2 heads of 64: 43 us, 0.37 of the copy rate, bound by what
+// lies between pieces of work (4000 cycles for a piece's 9000); one tree of 8 nodes over 1,000: 12 us.
 // Every wait is bounded: on expiry the CTA records a status word, drains and returns with its TMEM freed.
 #include "token_tree.cuh"
 
@@ -639,7 +644,7 @@ tree_attn_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
               settle();
               tmem_st_32x16(p_addr + x * 16, pk);
             };
-            if constexpr (REP > 1 && !S::APART) {  // the other copies' columns
+            if constexpr (REP > 1 && !S::APART) {  // the other copies' columns (over scores of this row: its own have to be in registers, as they are)
               const uint32_t none[16] = {};
 #pragma unroll
               for (int x = 0; x < 4; ++x)
