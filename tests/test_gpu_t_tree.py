@@ -824,3 +824,25 @@ def test_speculating_requests_keep_their_penalties():
             elif i % 4 == 3:
                 assert all(t % 50 == 7 for t in r.output_ids)
     e.shutdown()
+
+
+@pytest.mark.parametrize("speculate", [False, True])
+def test_the_largest_penalties_leave_a_distribution_on_the_gpu(speculate):
+    from slime_b200.engine.engine import Engine
+    from slime_b200.engine.server_args import ServerArgs
+    from slime_b200.models.config import ModelConfig
+
+    cfg = ModelConfig(num_layers=2, hidden_size=128, num_attention_heads=4, num_query_groups=2, kv_channels=64, ffn_hidden_size=256, vocab_size=512, rotary_base=1e4,
+                      tie_word_embeddings=False, mtp_num_layers=1, qk_layernorm=True, model_arch="Qwen3ForCausalLM")  # fmt: skip
+    kw = dict(speculative_algorithm="EAGLE", speculative_num_steps=3, speculative_num_draft_tokens=4) if speculate else {}
+    e = Engine(cfg, ServerArgs(page_size=16, max_running_requests=8, context_length=512, **kw), device="cuda", num_pages=400)
+    e.weights.init_random(0, std=0.2)
+    inf = math.inf
+    asks = [dict(frequency_penalty=s * 1e9, presence_penalty=s * 1e9, repetition_penalty=r, logit_bias={5: s * 1e9, 6: -s * 1e9, 7: -inf})
+            for s in (-1, 1) for r in (1e-9, 1e9)] + [dict(logit_bias={t: -inf for t in range(520) if t != 9}), {}]  # fmt: skip
+    for sampling in (dict(temperature=0), dict(temperature=1.0), dict(temperature=0.01), dict(temperature=1.0, top_p=0.9, top_k=20)):
+        reqs = e.generate([[1, 2, 3]] * len(asks), [dict(max_new_tokens=8, ignore_eos=True, **sampling, **a) for a in asks])
+        for r, a in zip(reqs, asks):
+            assert len(r.output_ids) == 8 and all(0 <= t < 512 for t in r.output_ids) and all(math.isfinite(x) for x in r.output_logprobs), (sampling, a, r.output_ids)
+        assert reqs[4].output_ids == [9] * 8 and not any(7 in r.output_ids for r in reqs[:4])
+    e.shutdown()
